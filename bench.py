@@ -1055,25 +1055,45 @@ def main():
         _ = model.prediction
         return model.loss_func
 
-    for _ in range(args.warmup):
-        step()
-    timer.reset(args.steps, args.warmup)
-    if world > 1:
-        dist.barrier()
-    torch.cuda.synchronize()
-    t0 = time.perf_counter()
-    for _ in range(args.steps):
-        loss = step()
-    torch.cuda.synchronize()
-    if world > 1:
-        dist.barrier()
-    elapsed = time.perf_counter() - t0
-    if world > 1:
-        tmax = torch.tensor([elapsed], device=device if dist.get_backend() == "nccl" else "cpu", dtype=torch.float64)
-        dist.all_reduce(tmax, op=dist.ReduceOp.MAX)
-        elapsed = float(tmax.item())
-    loss_val = float(loss)
-    ops.coop_check(device)
+    # Ranks that SHARE a GPU can starve each other's cooperative groups into the bounded wait (see the named workloads): then every
+    # rank takes the fall-back together and the whole measurement is made again.  One rank per GPU: the first attempt is the only one.
+    polls, ops.COOP_POLL_RAISES = ops.COOP_POLL_RAISES, ops.COOP_POLL_RAISES and world == 1
+    for attempt in range(3):
+        for _ in range(args.warmup):
+            step()
+        timer.reset(args.steps, args.warmup)
+        if world > 1:
+            dist.barrier()
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for _ in range(args.steps):
+            loss = step()
+        torch.cuda.synchronize()
+        if world > 1:
+            dist.barrier()
+        elapsed = time.perf_counter() - t0
+        if world > 1:
+            tmax = torch.tensor([elapsed], device=device if dist.get_backend() == "nccl" else "cpu", dtype=torch.float64)
+            dist.all_reduce(tmax, op=dist.ReduceOp.MAX)
+            elapsed = float(tmax.item())
+        loss_val = float(loss)
+        try:
+            ops.coop_check(device)
+            late = 0
+        except ops.CoopTimeout:
+            if world == 1:
+                raise
+            late = 1
+        if world > 1:
+            flag = torch.tensor([late], device=device if dist.get_backend() == "nccl" else "cpu", dtype=torch.int32)
+            dist.all_reduce(flag, op=dist.ReduceOp.MAX)
+            late = int(flag.item())
+        if not late:
+            break
+        if attempt == 2:
+            raise ops.CoopTimeout(ops._COOP_MSG)
+        ops.coop_fall_back(device)
+    ops.COOP_POLL_RAISES = polls
 
     totals = timer.totals()
     if rank == 0 and train:
