@@ -218,6 +218,11 @@ PROTOTYPES = {
     "avsi_lws_istft_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "avsi_lws_istft_f32": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_void_p,
                                    c_size_t, c_void_p]),
+    "avsi_layer_norm": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                c_int, c_float, c_void_p]),
+    "avsi_layer_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "avsi_layer_norm_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                    c_int64, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None
@@ -267,6 +272,21 @@ def require_cuda(*tensors):
 def stream_ptr():
     import torch
     return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def launch_on(device, name, *args):
+    """Call the entry point `name` with the current stream of `device` -- which need not be the current device -- behind its
+    arguments, and check its status."""
+    import torch
+    index = device.index
+    fn = getattr(lib(), name)
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != AVSI_OK:
+        check(status, name)
 
 
 def ptr(t):

@@ -1,0 +1,78 @@
+// Element types and lane sums shared by the kernels that take float32, bfloat16 and float16 tensors
+// (layer_norm.hip, scan.hip, causal_conv.hip, adamw.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+typedef __attribute__((ext_vector_type(2))) float avsi_f2;
+typedef __attribute__((ext_vector_type(4))) float avsi_f4;
+
+// One element type behind the codes avsi_dtype of the C ABI: rounding from fp32 is to nearest even in all of them.
+template <int CODE> struct avsi_type;
+template <> struct avsi_type<AVSI_F32> { typedef float T; };
+template <> struct avsi_type<AVSI_BF16> { typedef __bf16 T; };
+template <> struct avsi_type<AVSI_F16> { typedef _Float16 T; };
+
+static inline bool avsi_dtype_ok(int code) { return code == AVSI_F32 || code == AVSI_BF16 || code == AVSI_F16; }
+static inline int avsi_dtype_size(int code) { return code == AVSI_F32 ? 4 : 2; }
+
+// V consecutive elements as fp32.  gfx950 takes loads and stores of 16 bytes at any address that is aligned to the element, so rows
+// of odd width or pitch need no kernel of their own; `n` < V elements exist at the end of a row: those are taken one by one.
+template <typename T, int V> struct avsi_raw { T v[V]; };
+template <typename T, int V> __device__ __forceinline__ avsi_raw<T, V> avsi_load_raw(const T* __restrict__ p, int n) {
+    avsi_raw<T, V> r;
+    if (n >= V) {
+        __builtin_memcpy(&r, p, sizeof(r));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
+    }
+    return r;
+}
+template <typename T, int V> __device__ __forceinline__ void avsi_load(const T* __restrict__ p, int n, float (&f)[V]) {
+    const avsi_raw<T, V> r = avsi_load_raw<T, V>(p, n);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = (float)r.v[i];
+}
+template <typename T, int V> __device__ __forceinline__ void avsi_store(T* __restrict__ p, int n, const float (&f)[V]) {
+    avsi_raw<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = (T)f[i];
+    if (n >= V) {
+        __builtin_memcpy(p, &r, sizeof(r));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) p[i] = r.v[i];
+    }
+}
+
+// A lane permutation inside rows of 16 as a VALU operand (no LDS).
+template <int CTRL> __device__ __forceinline__ float avsi_dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// a[lanes 32 .. 63] <-> b[lanes 0 .. 31], and the same of the odd rows of a with the even rows of b.
+__device__ __forceinline__ void avsi_swap32(float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned x = r[0], y = r[1];
+    a = __builtin_bit_cast(float, x);
+    b = __builtin_bit_cast(float, y);
+}
+__device__ __forceinline__ void avsi_swap16(float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned x = r[0], y = r[1];
+    a = __builtin_bit_cast(float, x);
+    b = __builtin_bit_cast(float, y);
+}
+
+// Sum (or maximum) over every aligned group of G lanes, left in all of them; the order is fixed.
+struct avsi_add { static __device__ __forceinline__ float of(float a, float b) { return a + b; } };
+template <int G, typename OP = avsi_add> __device__ __forceinline__ float avsi_group(float v) {
+    if (G >= 2) v = OP::of(v, avsi_dpp<0xB1>(v));       // quad_perm [1, 0, 3, 2]
+    if (G >= 4) v = OP::of(v, avsi_dpp<0x4E>(v));       // quad_perm [2, 3, 0, 1]
+    if (G >= 8) v = OP::of(v, avsi_dpp<0x141>(v));      // row_half_mirror: the other quad of the eight
+    if (G >= 16) v = OP::of(v, avsi_dpp<0x140>(v));     // row_mirror: the other eight of the row
+    if (G >= 32) { float a = v, b = v; avsi_swap16(a, b); v = OP::of(a, b); }
+    if (G >= 64) { float a = v, b = v; avsi_swap32(a, b); v = OP::of(a, b); }
+    return v;
+}

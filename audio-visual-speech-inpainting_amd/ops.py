@@ -11,6 +11,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .sequence_ops import layer_norm, layer_norm_bwd   # noqa: F401
 
 
 def gemm(a, b, out=None, trans_a=False, trans_b=False, m=None, n=None, k=None, alpha=1.0, beta=0.0,

@@ -704,6 +704,27 @@ int avsi_tfrecord_files_decode_fixed_host(const char* const* paths, int count, i
                                           float* embedding, char* sample_paths, int sample_path_cap, float* labels,
                                           float* video, float* mask, int32_t* codes);
 
+/* ------------------------------------------------------------------------------------
+ * Layer norm over the last dimension of a [rows][cols] matrix, forward and backward (no reference counterpart: the
+ * reference normalises batches only, unet_layers.py:6-37).
+ *   mean = sum(x) / cols, var = sum((x - mean)^2) / cols, rstd = 1 / sqrt(var + eps), h = (x - mean) rstd,
+ *   y = h gamma + beta;   e = dy gamma, dx = rstd (e - mean(e) - h mean(e h)), dgamma = sum_rows dy h, dbeta = sum_rows dy.
+ *   x, y, dy, dx  elements of type `dtype` (avsi_dtype), unit stride along a row, row strides in elements, any alignment
+ *                 an element has; every output tensor distinct from the inputs
+ *   gamma, beta   [cols] of type `wdtype` (AVSI_F32, or the same as dtype); either may be NULL (1 and 0)
+ *   mean, rstd    [rows] float; dgamma, dbeta [cols] float, both NULL when they are not wanted
+ * All sums are fp32; outputs are rounded once, to nearest even.  The reduction over the rows is deterministic: partials
+ * in the workspace (avsi_layer_norm_bwd_workspace_bytes), no atomics.
+ * ------------------------------------------------------------------------------------ */
+typedef enum avsi_dtype { AVSI_F32 = 0, AVSI_BF16 = 1, AVSI_F16 = 2 } avsi_dtype;
+
+int avsi_layer_norm(const void* x, int64_t x_stride, int dtype, const void* gamma, const void* beta, int wdtype, void* y,
+                    int64_t y_stride, float* mean, float* rstd, int64_t rows, int cols, float eps, void* stream);
+size_t avsi_layer_norm_bwd_workspace_bytes(int64_t rows, int cols, int dtype);
+int avsi_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int dtype, const float* mean,
+                        const float* rstd, const void* gamma, int wdtype, void* dx, int64_t dx_stride, float* dgamma,
+                        float* dbeta, int64_t rows, int cols, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
