@@ -59,6 +59,17 @@ class GemmEpilogue(Structure):
                 ("row_map_bp", c_int32), ("row_map_t", c_int32), ("row_map_b", c_int32), ("k_zero", c_int32 * 4)]
 
 
+class ScanArgs(Structure):
+    """Mirror of ``avsi_scan_args`` (include/avsi_hip.h)."""
+    _fields_ = (
+        [(n, c_int32) for n in ("dtype", "batch", "time", "dim", "state", "groups", "softplus", "reserved")]
+        + [(n, c_void_p) for n in ("u", "dt", "z", "B", "C")]
+        + [(n, c_int64 * k) for n, k in (("u_stride", 2), ("dt_stride", 2), ("z_stride", 2), ("B_stride", 3), ("C_stride", 3))]
+        + [(n, c_void_p) for n in ("A", "D", "dt_bias", "state_in", "lengths", "out")] + [("out_stride", c_int64 * 2)]
+        + [(n, c_void_p) for n in ("state_out", "kept", "dout")] + [("dout_stride", c_int64 * 2)]
+        + [(n, c_void_p) for n in ("du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias")])
+
+
 # name -> (restype, argtypes); every symbol include/avsi_hip.h declares
 PROTOTYPES = {
     "avsi_abi_version": (c_int, []),
@@ -223,6 +234,20 @@ PROTOTYPES = {
     "avsi_layer_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "avsi_layer_norm_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                     c_int64, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "avsi_causal_conv": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64,
+                                 c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
+    "avsi_causal_conv_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "avsi_causal_conv_bwd": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                                     c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
+                                     c_size_t, c_void_p]),
+    "avsi_causal_conv_step": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int,
+                                      c_int, c_void_p]),
+    "avsi_selective_scan_kept_floats": (c_size_t, [POINTER(ScanArgs)]),
+    "avsi_selective_scan_workspace_bytes": (c_size_t, [POINTER(ScanArgs)]),
+    "avsi_selective_scan": (c_int, [POINTER(ScanArgs), c_void_p, c_size_t, c_void_p]),
+    "avsi_selective_scan_bwd_workspace_bytes": (c_size_t, [POINTER(ScanArgs)]),
+    "avsi_selective_scan_bwd": (c_int, [POINTER(ScanArgs), c_void_p, c_size_t, c_void_p]),
+    "avsi_selective_scan_step": (c_int, [POINTER(ScanArgs), c_void_p]),
 }
 
 _lib = None

@@ -76,3 +76,18 @@ template <int G, typename OP = avsi_add> __device__ __forceinline__ float avsi_g
     if (G >= 64) { float a = v, b = v; avsi_swap32(a, b); v = OP::of(a, b); }
     return v;
 }
+
+// Functions of the gates, to about 2 ulp.  log(1 + e) for 0 <= e <= 1 as 2 atanh(e / (2 + e)), by its series: with s <= 1 / 3 the
+// first term left out is below 2e-9 of the sum, and small e keep their relative accuracy (1 + e would round them away).
+__device__ __forceinline__ float avsi_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + expf(-x)); }
+__device__ __forceinline__ float avsi_softplus(float x) {
+    const float e = expf(-fabsf(x));
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e), p = s * s;
+    float q = fmaf(p, 1.f / 15.f, 1.f / 13.f);
+    q = fmaf(p, q, 1.f / 11.f);
+    q = fmaf(p, q, 1.f / 9.f);
+    q = fmaf(p, q, 1.f / 7.f);
+    q = fmaf(p, q, 1.f / 5.f);
+    q = fmaf(p, q, 1.f / 3.f);
+    return fmaxf(x, 0.f) + 2.f * fmaf(s * p, q, s);
+}

@@ -11,7 +11,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from .sequence_ops import layer_norm, layer_norm_bwd   # noqa: F401
+from .sequence_ops import (causal_conv, causal_conv_bwd, causal_conv_step, layer_norm, layer_norm_bwd,   # noqa: F401
+                           selective_scan, selective_scan_bwd, selective_scan_step)
 
 
 def gemm(a, b, out=None, trans_a=False, trans_b=False, m=None, n=None, k=None, alpha=1.0, beta=0.0,

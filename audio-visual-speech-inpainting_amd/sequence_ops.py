@@ -136,3 +136,242 @@ def layer_norm_bwd(dy, x, mean, rstd, gamma=None, want_wgrad=True, dx=None):
                        0 if gamma is None else _CODES[gamma.dtype], dx.data_ptr(), dxs, p, None if p is None else p + 4 * C, M, C, _p(ws),
                        nbytes)
     return (dx, grads[0], grads[1]) if want_wgrad else (dx, None, None)
+
+
+# -------------------------------------------------------------------------------------------------------- causal convolution
+def _seq(what, name, t, shape, dtype):
+    """(batch stride, time stride) of a [batch, time, dim] tensor; its channels lie next to each other."""
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        _bad("%s: %s must be %s of shape %s, not %s of %s", what, name, dtype, shape, t.dtype, tuple(t.shape))
+    if shape[2] > 1 and t.stride(2) != 1:
+        _bad("%s: %s must have unit stride along its channels", what, name)
+    return t.stride(0), t.stride(1)
+
+
+def _vector(what, name, t, *shape):
+    """A contiguous float32 weight."""
+    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
+        _bad("%s: %s must be contiguous float32 of shape %s", what, name, shape)
+
+
+def _state(what, t, shape, dtype):
+    if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous()):
+        _bad("%s: state must be contiguous %s of shape %s", what, dtype, shape)
+
+
+def _lengths(what, t, batch):
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous()):
+        _bad("%s: lengths must be %d contiguous int32 values", what, batch)
+
+
+def _conv_args(what, x, w, bias, dims):
+    if x.dtype not in _CODES or x.dim() != dims:
+        _bad("%s: x must be a float32, bfloat16 or float16 tensor of %d dimensions", what, dims)
+    D = x.shape[-1]
+    if w.dim() != 2 or not 2 <= w.shape[1] <= 8 or D < 1:
+        _bad("%s: w must be [channels, taps] with 2 to 8 taps", what)
+    _vector(what, "w", w, D, w.shape[1])
+    _vector(what, "bias", bias, D)
+    return x.shape[0], D, w.shape[1]
+
+
+def causal_conv(x, w, bias=None, silu=True, state=None, lengths=None, want_state=False):
+    """(y, new_state): the short causal convolution along time, one filter per channel (avsi_causal_conv).
+
+    x [batch, time, channels], w [channels, taps] and bias [channels] float32; y = silu(pre) or pre.  state [batch, taps - 1, channels]
+    of x's type: the inputs in front of x (None: zeros).  lengths: int32, steps of each sequence (values outside 0 .. time are
+    clamped); behind them y is zero and x is not read.  new_state (None unless asked for): the state behind each sequence's end, for
+    the next piece or ``causal_conv_step``."""
+    B, D, K = _conv_args("causal_conv", x, w, bias, 3)
+    T = x.shape[1]
+    xb, xt = _seq("causal_conv", "x", x, (B, T, D), x.dtype)
+    _state("causal_conv", state, (B, K - 1, D), x.dtype)
+    _lengths("causal_conv", lengths, B)
+    dev = _device("causal_conv", x, w, bias, state, lengths)
+    y = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+    new = torch.empty((B, K - 1, D), dtype=x.dtype, device=dev) if want_state else None
+    if B and T:
+        _lib.launch_on(dev, "avsi_causal_conv", x.data_ptr(), xb, xt, _CODES[x.dtype], w.data_ptr(), _p(bias), int(silu), _p(state),
+                       _p(lengths), y.data_ptr(), T * D, D, _p(new), B, T, D, K)
+    elif want_state and B:
+        new.zero_() if state is None else new.copy_(state)
+    return y, new
+
+
+def causal_conv_bwd(dy, x, w, bias=None, silu=True, state=None, lengths=None, want_wgrad=True):
+    """(dx, dw, dbias) of ``causal_conv`` (avsi_causal_conv_bwd): dy of x's shape and type, the other arguments as in the forward
+    call.  dw, dbias: float32, None with ``want_wgrad=False`` (dbias also without a bias).  No gradient goes into the state."""
+    B, D, K = _conv_args("causal_conv_bwd", x, w, bias, 3)
+    T = x.shape[1]
+    xb, xt = _seq("causal_conv_bwd", "x", x, (B, T, D), x.dtype)
+    gb, gt = _seq("causal_conv_bwd", "dy", dy, (B, T, D), x.dtype)
+    _state("causal_conv_bwd", state, (B, K - 1, D), x.dtype)
+    _lengths("causal_conv_bwd", lengths, B)
+    dev = _device("causal_conv_bwd", x, dy, w, bias, state, lengths)
+    dx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+    dw = torch.empty((D, K), dtype=torch.float32, device=dev) if want_wgrad else None
+    dbias = torch.empty(D, dtype=torch.float32, device=dev) if want_wgrad and bias is not None else None
+    if B and T:
+        code = _CODES[x.dtype]
+        nbytes = _lib.lib().avsi_causal_conv_bwd_workspace_bytes(code, B, T, D, K) if want_wgrad else 0
+        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
+        _lib.launch_on(dev, "avsi_causal_conv_bwd", dy.data_ptr(), gb, gt, x.data_ptr(), xb, xt, code, w.data_ptr(), _p(bias), int(silu),
+                       _p(state), _p(lengths), dx.data_ptr(), T * D, D, _p(dw), _p(dbias), B, T, D, K, _p(ws), nbytes)
+    else:
+        for t in (dw, dbias):
+            if t is not None:
+                t.zero_()
+    return dx, dw, dbias
+
+
+def causal_conv_step(x, w, bias=None, silu=True, *, state):
+    """y [batch, channels] of one token per sequence (avsi_causal_conv_step): x [batch, channels]; ``state`` [batch, taps - 1, channels]
+    of x's type moves on by one input, in place."""
+    B, D, K = _conv_args("causal_conv_step", x, w, bias, 2)
+    if D > 1 and x.stride(1) != 1:
+        _bad("causal_conv_step: x must have unit stride along its channels")
+    _state("causal_conv_step", state, (B, K - 1, D), x.dtype)
+    if _overlap(x, state):
+        _bad("causal_conv_step: x must not be part of the state")
+    dev = _device("causal_conv_step", x, w, bias, state)
+    y = torch.empty((B, D), dtype=x.dtype, device=dev)
+    if B:
+        _lib.launch_on(dev, "avsi_causal_conv_step", x.data_ptr(), x.stride(0), _CODES[x.dtype], w.data_ptr(), _p(bias), int(silu),
+                       state.data_ptr(), y.data_ptr(), D, B, D, K)
+    return y
+
+
+# ------------------------------------------------------------------------------------------------------------ selective scan
+def _groups(what, name, t, lead, N, dtype):
+    """(groups, strides) of B or C: [..., groups, state], or [..., state] for one group."""
+    n = len(lead)
+    if t.dtype != dtype or t.dim() not in (n + 1, n + 2) or tuple(t.shape[:n]) != lead or t.shape[-1] != N:
+        _bad("%s: %s must be %s of shape %s + [groups, %d]", what, name, dtype, lead, N)
+    if N > 1 and t.stride(-1) != 1:
+        _bad("%s: %s must have unit stride along its states", what, name)
+    if t.dim() == n + 1:
+        return 1, (t.stride(0), t.stride(1) if n == 2 else 0, 0)
+    return t.shape[n], (t.stride(0), t.stride(1) if n == 2 else 0, t.stride(n))
+
+
+def _scan_args(what, u, dt, A, B, C, D, z, dt_bias, softplus, lead):
+    """The checked operands that all forms of the scan take, as avsi_scan_args."""
+    if u.dtype not in _CODES or u.dim() != len(lead) + 1 or u.shape[-1] < 1:
+        _bad("%s: u must be a float32, bfloat16 or float16 tensor of %d dimensions", what, len(lead) + 1)
+    dim, dtype = u.shape[-1], u.dtype
+    if A.dim() != 2 or not 1 <= A.shape[1] <= 64:
+        _bad("%s: A must be [channels, states] with 1 to 64 states", what)
+    N = A.shape[1]
+    _vector(what, "A", A, dim, N)
+    _vector(what, "D", D, dim)
+    _vector(what, "dt_bias", dt_bias, dim)
+    a = _lib.ScanArgs(_CODES[dtype], lead[0], lead[1] if len(lead) == 2 else 1, dim, N, 1, int(softplus))
+    if lead[0] > 65535:
+        _bad("%s: at most 65535 sequences", what)
+    for name, t in (("u", u), ("dt", dt), ("z", z)):
+        if t is None:
+            continue
+        if t.dtype != dtype or t.shape != u.shape:
+            _bad("%s: %s must be %s of shape %s, not %s of %s", what, name, dtype, tuple(u.shape), t.dtype, tuple(t.shape))
+        if dim > 1 and t.stride(-1) != 1:
+            _bad("%s: %s must have unit stride along its channels", what, name)
+        setattr(a, name, t.data_ptr())
+        s = getattr(a, name + "_stride")
+        s[0], s[1] = t.stride(0), t.stride(1) if len(lead) == 2 else 0
+    G, a.B_stride = _groups(what, "B", B, lead, N, dtype)
+    G2, a.C_stride = _groups(what, "C", C, lead, N, dtype)
+    if G != G2 or G < 1 or dim % G:
+        _bad("%s: B and C must have one number of groups, which divides the %d channels", what, dim)
+    a.groups, a.B, a.C, a.A, a.D, a.dt_bias = G, B.data_ptr(), C.data_ptr(), A.data_ptr(), _p(D), _p(dt_bias)
+    return a, N
+
+
+def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, state=None, lengths=None, want_state=False, keep=False):
+    """(out, new_state, kept): the selective state-space scan of whole sequences (avsi_selective_scan).
+
+        delta = softplus(dt + dt_bias),  h[t] = exp(delta A) h[t - 1] + delta u B[t],  y = C[t] . h[t] + D u,  out = y silu(z)
+
+    u, dt, z [batch, time, channels]; B, C [batch, time, groups, states] ([batch, time, states] for one group) of u's type; A
+    [channels, states], D, dt_bias [channels] float32; D, z, dt_bias may be None.  ``softplus=False`` takes dt + dt_bias as it is.
+    state: float32 [batch, channels, states] in front of the first step (None: zeros).  lengths: int32 steps per sequence (clamped to
+    0 .. time); behind them out is zero, the state stands still and nothing is read.  new_state (None unless asked for): float32, the
+    state behind each sequence's end.  kept (None unless ``keep``): what ``selective_scan_bwd`` needs, 4 bytes per channel and step
+    at 16 states."""
+    what = "selective_scan"
+    if u.dim() != 3:
+        _bad("%s: u must be [batch, time, channels]", what)
+    bsz, T, dim = u.shape
+    a, N = _scan_args(what, u, dt, A, B, C, D, z, dt_bias, softplus, (bsz, T))
+    _state(what, state, (bsz, dim, N), torch.float32)
+    _lengths(what, lengths, bsz)
+    dev = _device(what, u, dt, A, B, C, D, z, dt_bias, state, lengths)
+    out = torch.empty((bsz, T, dim), dtype=u.dtype, device=dev)
+    new = torch.empty((bsz, dim, N), dtype=torch.float32, device=dev) if want_state else None
+    kept = None
+    if not (bsz and T):
+        if want_state and bsz:
+            new.zero_() if state is None else new.copy_(state)
+        return out, new, torch.empty(0, dtype=torch.float32, device=dev) if keep else None
+    L = _lib.lib()
+    if keep:
+        kept = torch.empty(L.avsi_selective_scan_kept_floats(a), dtype=torch.float32, device=dev)
+    a.state_in, a.lengths, a.out, a.state_out, a.kept = _p(state), _p(lengths), out.data_ptr(), _p(new), _p(kept)
+    a.out_stride[0], a.out_stride[1] = T * dim, dim
+    nbytes = L.avsi_selective_scan_workspace_bytes(a)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
+    _lib.launch_on(dev, "avsi_selective_scan", a, _p(ws), nbytes)
+    return out, new, kept
+
+
+def selective_scan_bwd(dout, u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, *, kept, state=None, lengths=None):
+    """(du, ddt, dA, dB, dC, dD, dz, ddt_bias) of ``selective_scan`` (avsi_selective_scan_bwd): dout of u's shape and type, ``kept``
+    from the forward call with ``keep=True``, the other arguments as there.  du, ddt, dz, dB, dC have the inputs' type; dA, dD,
+    ddt_bias are float32; what belongs to an argument that is None is None.  No gradient goes into the state."""
+    what = "selective_scan_bwd"
+    if u.dim() != 3:
+        _bad("%s: u must be [batch, time, channels]", what)
+    bsz, T, dim = u.shape
+    a, N = _scan_args(what, u, dt, A, B, C, D, z, dt_bias, softplus, (bsz, T))
+    a.dout_stride[0], a.dout_stride[1] = _seq(what, "dout", dout, (bsz, T, dim), u.dtype)
+    _state(what, state, (bsz, dim, N), torch.float32)
+    _lengths(what, lengths, bsz)
+    L = _lib.lib()
+    if kept.dtype != torch.float32 or not kept.is_contiguous() or kept.numel() != L.avsi_selective_scan_kept_floats(a):
+        _bad("%s: kept must be what selective_scan returned with keep=True for these operands", what)
+    dev = _device(what, u, dt, A, B, C, D, z, dt_bias, dout, kept, state, lengths)
+    du, ddt = torch.empty((2, bsz, T, dim), dtype=u.dtype, device=dev).unbind(0)
+    dz = None if z is None else torch.empty((bsz, T, dim), dtype=u.dtype, device=dev)
+    dB, dC = torch.empty(B.shape, dtype=u.dtype, device=dev), torch.empty(C.shape, dtype=u.dtype, device=dev)
+    dA = torch.empty((dim, N), dtype=torch.float32, device=dev)
+    dD = None if D is None else torch.empty(dim, dtype=torch.float32, device=dev)
+    ddt_bias = None if dt_bias is None else torch.empty(dim, dtype=torch.float32, device=dev)
+    if bsz and T:
+        a.lengths, a.kept, a.dout = _p(lengths), kept.data_ptr(), dout.data_ptr()
+        a.du, a.ddt, a.dz, a.dB, a.dC = du.data_ptr(), ddt.data_ptr(), _p(dz), dB.data_ptr(), dC.data_ptr()
+        a.dA, a.dD, a.ddt_bias = dA.data_ptr(), _p(dD), _p(ddt_bias)
+        nbytes = L.avsi_selective_scan_bwd_workspace_bytes(a)
+        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
+        _lib.launch_on(dev, "avsi_selective_scan_bwd", a, ws.data_ptr(), nbytes)
+    else:
+        for t in (dA, dD, ddt_bias):
+            if t is not None:
+                t.zero_()
+    return du, ddt, dA, dB, dC, dD, dz, ddt_bias
+
+
+def selective_scan_step(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, *, state):
+    """out [batch, channels] of one token per sequence (avsi_selective_scan_step): u, dt, z [batch, channels]; B, C [batch, groups,
+    states] or [batch, states]; ``state`` float32 [batch, channels, states] moves on by one step, in place."""
+    what = "selective_scan_step"
+    if u.dim() != 2:
+        _bad("%s: u must be [batch, channels]", what)
+    bsz, dim = u.shape
+    a, N = _scan_args(what, u, dt, A, B, C, D, z, dt_bias, softplus, (bsz,))
+    _state(what, state, (bsz, dim, N), torch.float32)
+    dev = _device(what, u, dt, A, B, C, D, z, dt_bias, state)
+    out = torch.empty((bsz, dim), dtype=u.dtype, device=dev)
+    if bsz:
+        a.out, a.state_out = out.data_ptr(), state.data_ptr()
+        a.out_stride[0] = dim
+        _lib.launch_on(dev, "avsi_selective_scan_step", a)
+    return out

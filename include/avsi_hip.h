@@ -725,6 +725,74 @@ int avsi_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_
                         const float* rstd, const void* gamma, int wdtype, void* dx, int64_t dx_stride, float* dgamma,
                         float* dbeta, int64_t rows, int cols, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Short causal convolution along time, one filter of `taps` = 2 .. 8 per channel, in front of a selective scan (no
+ * reference counterpart).
+ *   pre[b][t][d] = bias[d] + sum_k w[d][k] x[b][t - taps + 1 + k][d];  y = silu ? pre sigmoid(pre) : pre
+ *   x, y, dy, dx   `dtype`, [batch][time][dim] with strides of batch and time in elements, unit stride along the channels
+ *   w [dim][taps], bias [dim] (or NULL), dw, dbias: float
+ *   state          `dtype` [batch][taps - 1][dim]: the inputs in front of x[0], oldest first; NULL: zeros.  It is a
+ *                  constant of the backward pass
+ *   lengths        device int32 [batch] or NULL: sequence b has min(max(lengths[b], 0), time) steps; behind them y and dx
+ *                  are zero and x, dy are not read
+ *   state_out      `dtype` [batch][taps - 1][dim] or NULL: the last inputs in front of each sequence's end (not `state`)
+ * The step takes one token per sequence ([batch][dim], stride of batch) and moves `state` on in place.
+ * dw and dbias may be NULL (dw only together with dbias); their sums have a fixed order, no atomics.
+ * ------------------------------------------------------------------------------------ */
+int avsi_causal_conv(const void* x, int64_t x_stride_b, int64_t x_stride_t, int dtype, const float* w, const float* bias,
+                     int silu, const void* state, const int32_t* lengths, void* y, int64_t y_stride_b, int64_t y_stride_t,
+                     void* state_out, int batch, int time, int dim, int taps, void* stream);
+size_t avsi_causal_conv_bwd_workspace_bytes(int dtype, int batch, int time, int dim, int taps);
+int avsi_causal_conv_bwd(const void* dy, int64_t dy_stride_b, int64_t dy_stride_t, const void* x, int64_t x_stride_b,
+                         int64_t x_stride_t, int dtype, const float* w, const float* bias, int silu, const void* state,
+                         const int32_t* lengths, void* dx, int64_t dx_stride_b, int64_t dx_stride_t, float* dw, float* dbias,
+                         int batch, int time, int dim, int taps, void* workspace, size_t workspace_bytes, void* stream);
+int avsi_causal_conv_step(const void* x, int64_t x_stride_b, int dtype, const float* w, const float* bias, int silu,
+                          void* state, void* y, int64_t y_stride_b, int batch, int dim, int taps, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Selective state-space scan (no reference counterpart; the recurrence next to it is the LSTM, models.py:89-115).
+ *   delta = softplus ? log(1 + exp(dt + dt_bias)) : dt + dt_bias;  a = exp(delta A);  h[t] = a h[t - 1] + delta u B[t];
+ *   y = sum_n C[t][n] h[t][n] + D u;  out = z ? y z sigmoid(z) : y
+ *   u, dt, z, dout   `dtype` [batch][time][dim], strides {batch, time}, unit stride along the channels; z may be NULL
+ *   B, C             `dtype` [batch][time][groups][state], strides {batch, time, group}, unit stride along the states;
+ *                    channel d belongs to group d / (dim / groups)
+ *   A [dim][state], D [dim] or NULL (0), dt_bias [dim] or NULL (0): float.  state <= 64, batch <= 65535
+ *   state_in         float [batch][dim][state] or NULL (zeros), a constant of the backward pass; state_out: the state at each
+ *                    sequence's end, or NULL (not state_in)
+ *   lengths          as for the convolution: behind its length a sequence's state stands still, out and all gradients are
+ *                    zero, and nothing is read
+ *   out              `dtype`, strides {batch, time}
+ *   kept             forward: NULL, or room for avsi_selective_scan_kept_floats() floats -- the states the backward pass
+ *                    starts its tiles from; backward: what the forward call left there
+ *   du, ddt, dz      `dtype` [batch][time][dim] contiguous (dz NULL exactly if z is); dB, dC: `dtype`
+ *                    [batch][time][groups][state] contiguous; dA [dim][state], dD [dim], ddt_bias [dim]: float (dD,
+ *                    ddt_bias may be NULL)
+ * States, sums and statistics are float; every sum has a fixed order.  The step takes one token per sequence (time = 1,
+ * strides of time unused) and moves the states in `state_out` on in place (state_in, lengths, kept unused).
+ * ------------------------------------------------------------------------------------ */
+typedef struct avsi_scan_args {
+    int32_t dtype, batch, time, dim, state, groups, softplus, reserved;
+    const void *u, *dt, *z, *B, *C;
+    int64_t u_stride[2], dt_stride[2], z_stride[2], B_stride[3], C_stride[3];
+    const float *A, *D, *dt_bias, *state_in;
+    const int32_t* lengths;
+    void* out;
+    int64_t out_stride[2];
+    float *state_out, *kept;
+    const void* dout;
+    int64_t dout_stride[2];
+    void *du, *ddt, *dz, *dB, *dC;
+    float *dA, *dD, *ddt_bias;
+} avsi_scan_args;
+
+size_t avsi_selective_scan_kept_floats(const avsi_scan_args* args);
+size_t avsi_selective_scan_workspace_bytes(const avsi_scan_args* args);
+int avsi_selective_scan(const avsi_scan_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t avsi_selective_scan_bwd_workspace_bytes(const avsi_scan_args* args);
+int avsi_selective_scan_bwd(const avsi_scan_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int avsi_selective_scan_step(const avsi_scan_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
