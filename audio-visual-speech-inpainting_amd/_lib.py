@@ -70,6 +70,12 @@ class ScanArgs(Structure):
         + [(n, c_void_p) for n in ("du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias")])
 
 
+class AdamwTensor(Structure):
+    """Mirror of ``avsi_adamw_tensor`` (include/avsi_hip.h)."""
+    _fields_ = ([(n, c_void_p) for n in ("w", "grad", "copy", "m", "v", "m_scale", "v_scale")]
+                + [("numel", c_int64), ("weight_decay", c_float), ("grad_dtype", ctypes.c_int16), ("copy_dtype", ctypes.c_int16)])
+
+
 # name -> (restype, argtypes); every symbol include/avsi_hip.h declares
 PROTOTYPES = {
     "avsi_abi_version": (c_int, []),
@@ -248,6 +254,8 @@ PROTOTYPES = {
     "avsi_selective_scan_bwd_workspace_bytes": (c_size_t, [POINTER(ScanArgs)]),
     "avsi_selective_scan_bwd": (c_int, [POINTER(ScanArgs), c_void_p, c_size_t, c_void_p]),
     "avsi_selective_scan_step": (c_int, [POINTER(ScanArgs), c_void_p]),
+    "avsi_adamw": (c_int, [POINTER(AdamwTensor), c_int, c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_int64,
+                           ctypes.c_double, c_void_p, c_int, c_void_p]),
 }
 
 _lib = None

@@ -11,6 +11,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .optim_ops import AdamwPlan, adamw   # noqa: F401
 from .sequence_ops import (causal_conv, causal_conv_bwd, causal_conv_step, layer_norm, layer_norm_bwd,   # noqa: F401
                            selective_scan, selective_scan_bwd, selective_scan_step)
 

@@ -793,6 +793,30 @@ size_t avsi_selective_scan_bwd_workspace_bytes(const avsi_scan_args* args);
 int avsi_selective_scan_bwd(const avsi_scan_args* args, void* workspace, size_t workspace_bytes, void* stream);
 int avsi_selective_scan_step(const avsi_scan_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * One AdamW step (Adam with decoupled weight decay) over `count` tensors, `step` 1-based, next to avsi_adam_tf_f32:
+ *   g = grad grad_scale; m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2;
+ *   w -= lr (m / (1 - beta1^step) / (sqrt(v / (1 - beta2^step)) + eps) + weight_decay w); copy = w in its type, if not NULL
+ *   bits 32: m, v float.  bits 8: one byte per value, e4m3 codes of m / m_scale and of sqrt(v) / v_scale, where block k of
+ *   256 consecutive values of a tensor has the scales m_scale[k] = max|m| / 448, v_scale[k] = max sqrt(v) / 448; a value of
+ *   v above zero keeps at least the code of 2^-9.  A block that holds a non-finite moment decodes to NaN.
+ * `tensors` is a HOST array (read during the call, its pointers are device pointers; numel 0 is skipped); the tensors must
+ * not share memory.  `skip` as for avsi_adam_tf_guarded_f32: with any of its words non-zero nothing is written.
+ * ------------------------------------------------------------------------------------ */
+typedef struct avsi_adamw_tensor {
+    float* w;
+    const void* grad;        /* avsi_dtype grad_dtype */
+    void* copy;              /* NULL, or avsi_dtype copy_dtype */
+    void *m, *v;
+    float *m_scale, *v_scale;
+    int64_t numel;
+    float weight_decay;
+    int16_t grad_dtype, copy_dtype;
+} avsi_adamw_tensor;
+
+int avsi_adamw(const avsi_adamw_tensor* tensors, int count, int bits, double lr, double beta1, double beta2, double eps,
+               int64_t step, double grad_scale, const float* skip, int n_skip, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
