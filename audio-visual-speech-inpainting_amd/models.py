@@ -58,6 +58,25 @@ class BLSTMVariables:
         self.adam_v = None
         self.global_step = 0
         self.version = 0
+        self._adamw = None
+
+    def adamw_plan(self, grad, weight_decay):
+        """The AdamW plan over these variables (ops.AdamwPlan on views of ``flat`` and of the slots ``adam_m`` / ``adam_v``, which
+        checkpoints hold), reading the flat gradient ``grad``: matrices decay, vectors (biases) do not.  Made again when a
+        restored checkpoint has replaced a buffer."""
+        if self.adam_m is None:
+            self.adam_m = torch.zeros_like(self.flat)
+        if self.adam_v is None:
+            self.adam_v = torch.zeros_like(self.flat)
+        cut = lambda t: [t[off:off + int(np.prod(shape))] for _, shape, off in self.layout.ref_entries]                # noqa: E731
+        key = (self.flat.data_ptr(), self.adam_m.data_ptr(), self.adam_v.data_ptr(), weight_decay)
+        if self._adamw is None or self._adamw[0] != key:
+            decay = [weight_decay if len(shape) > 1 else 0.0 for _, shape, _ in self.layout.ref_entries]
+            self._adamw = (key, ops.AdamwPlan(cut(self.flat), cut(grad), weight_decay=decay,
+                                              state={'m': cut(self.adam_m), 'v': cut(self.adam_v)}))
+        else:
+            self._adamw[1].set_grads(cut(grad))
+        return self._adamw[1]
 
     @property
     def flat(self):
@@ -225,6 +244,7 @@ class StackedBLSTMModel(object):
         self.is_training = is_training
         self.batch_size = config.get('batch_size', 1)
         self.regularization = config['l2']
+        self.weight_decay = config.get('weight_decay', 0.01)      # optimizer_type adamw only
         self.var_scope = None
         self.rows_per_wg = int(config.get('rows_per_wg', 0))   # 0 = kernel picks 32/64 from the batch
         # 'f32' (default: exact fp32 fma chains on the fp32 matrix cores) or 'bf16x3' (EXPLORATORY: the layer input
@@ -837,7 +857,8 @@ class StackedBLSTMModel(object):
         """The optimiser update of ``train_op`` (reference models.py:168-179) with a gradient the caller hands in: ``g`` is
         the flat reference-layout gradient SUMMED over ``world`` equal shares (the update divides by it), ``guard`` the step
         guard's device words (any non-zero word leaves variables and slots alone).  Every optimizer_type runs as one guarded
-        HIP launch: TF-Adam with the CONSTANT starter rate, sgd / momentum 0.9 with the staircase-decayed rate."""
+        HIP launch: TF-Adam with the CONSTANT starter rate, sgd / momentum 0.9 / adamw with the staircase-decayed
+        rate."""
         v = self.variables
         step = v.global_step + 1
         l2 = float(self.regularization or 0.0)
@@ -855,8 +876,14 @@ class StackedBLSTMModel(object):
                     v.adam_m = torch.zeros_like(v.flat)         # the 'Momentum' slot
                 accum = v.adam_m
             ops.sgd_momentum(v.flat, g, accum, self.learning_rate, momentum=0.9, grad_scale=1.0 / world, l2=l2, skip=guard)
+        elif self.optimizer_choice == 'adamw':
+            # (no reference counterpart) decoupled weight decay on the matrices, key weight_decay, with the staircase-decayed rate
+            if l2:
+                raise ValueError("optimizer_type adamw decays the weights by weight_decay: l2 must be 0")
+            plan = v.adamw_plan(g, float(self.weight_decay))
+            ops.adamw(plan, step, self.learning_rate, grad_scale=1.0 / world, skip=guard)
         else:
-            print('Optimizer must be either sgd, momentum or adam. Closing...')
+            print('Optimizer must be either sgd, momentum, adam or adamw. Closing...')
             sys.exit(1)
         v.global_step = step
         v.repack()
