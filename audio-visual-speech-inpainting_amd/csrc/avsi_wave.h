@@ -47,6 +47,55 @@ template <typename T, int V> __device__ __forceinline__ void avsi_store(T* __res
     }
 }
 
+// Four elements as they lie in memory, in 32-bit words: a load of them that is in flight stays one register group, where an array of
+// 16-bit elements is taken apart (and waited for) at once.
+template <typename T> struct avsi_quad {
+    typedef __attribute__((ext_vector_type(sizeof(T)))) unsigned V;
+    V v;
+    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(&v, p, sizeof(v)); }
+    __device__ __forceinline__ void get(float (&f)[4]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = __builtin_bit_cast(float, (unsigned)v[i]);
+        } else if constexpr (__is_same(T, __bf16)) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                f[2 * i] = __builtin_bit_cast(float, (unsigned)v[i] << 16);
+                f[2 * i + 1] = __builtin_bit_cast(float, (unsigned)v[i] & 0xffff0000u);
+            }
+        } else {
+            typedef __attribute__((ext_vector_type(2))) _Float16 half2;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const half2 h = __builtin_bit_cast(half2, (unsigned)v[i]);
+                f[2 * i] = (float)h[0], f[2 * i + 1] = (float)h[1];
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float (&f)[4]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(unsigned, f[i]);
+        } else {
+            typedef __attribute__((ext_vector_type(2))) T Pair;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) v[i] = __builtin_bit_cast(unsigned, Pair{(T)f[2 * i], (T)f[2 * i + 1]});
+        }
+    }
+    // the first n of them
+    __device__ __forceinline__ void store(T* p, int n) const {
+        if (n >= 4) {
+            __builtin_memcpy(p, &v, sizeof(v));
+            return;
+        }
+        T e[4];
+        __builtin_memcpy(e, &v, sizeof(v));
+        if (n > 0) p[0] = e[0];
+        if (n > 1) p[1] = e[1];
+        if (n > 2) p[2] = e[2];
+    }
+};
+
 // A lane permutation inside rows of 16 as a VALU operand (no LDS).
 template <int CTRL> __device__ __forceinline__ float avsi_dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -77,11 +126,16 @@ template <int G, typename OP = avsi_add> __device__ __forceinline__ float avsi_g
     return v;
 }
 
-// Functions of the gates, to about 2 ulp.  log(1 + e) for 0 <= e <= 1 as 2 atanh(e / (2 + e)), by its series: with s <= 1 / 3 the
-// first term left out is below 2e-9 of the sum, and small e keep their relative accuracy (1 + e would round them away).
-__device__ __forceinline__ float avsi_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + expf(-x)); }
+// Functions of the gates, to a few ulp, on the hardware's base-2 exponential.  In softplus x log2 e is carried in two words; then
+// log(1 + e) for 0 <= e <= 1 is 2 atanh(e / (2 + e)), by its series: with s <= 1 / 3 the first term left out is below 2e-9 of the
+// sum, and small e keep their relative accuracy (1 + e would round them away).  A NaN comes out as one.
+__device__ __forceinline__ float avsi_sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));
+}
 __device__ __forceinline__ float avsi_softplus(float x) {
-    const float e = expf(-fabsf(x));
+    const float y = fmaxf(-fabsf(x), -120.f);
+    const float hi = y * 1.44269504088896340736f, lo = fmaf(y, 1.92596299112661746887e-8f, fmaf(y, 1.44269504088896340736f, -hi));
+    const float r = __builtin_amdgcn_exp2f(hi), e = fmaf(r, lo * 0.693147180559945309f, r);
     const float s = e * __builtin_amdgcn_rcpf(2.f + e), p = s * s;
     float q = fmaf(p, 1.f / 15.f, 1.f / 13.f);
     q = fmaf(p, q, 1.f / 11.f);
@@ -89,5 +143,5 @@ __device__ __forceinline__ float avsi_softplus(float x) {
     q = fmaf(p, q, 1.f / 7.f);
     q = fmaf(p, q, 1.f / 5.f);
     q = fmaf(p, q, 1.f / 3.f);
-    return fmaxf(x, 0.f) + 2.f * fmaf(s * p, q, s);
+    return (x < 0.f ? 0.f : x) + 2.f * fmaf(s * p, q, s);
 }

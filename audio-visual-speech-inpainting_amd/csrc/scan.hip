@@ -39,11 +39,11 @@ struct Scan {
     float* state_out;
     const int32_t* lengths;
     void* out;
-    float* kept;                     // [batch][tiles][dim][4 LN]
+    float* kept;                     // [batch][tiles][dim][NP]
     void *du, *ddt, *dz;             // [batch][time][dim]
-    float *part_bc, *part_w;         // [batch][time][groups][blocks][2][4 LN], [batch * chunks][partial_stride]
-    float *ends, *sums;              // [batch][chunks][dim][4 LN], [batch][chunks][dim]
-    int batch, T, dim, N, groups, softplus, chunk, chunks, blocks;     // chunk: steps, a multiple of TT; blocks: per group
+    float *part_bc, *part_w;         // [batch][time][groups][blocks][2][NP], [batch * chunks][partial_stride]
+    float *ends, *sums;              // [batch][chunks][dim][NP], [batch][chunks][dim]
+    int batch, T, dim, N, NP, groups, softplus, gated, chunk, chunks, blocks;     // chunk: steps, a multiple of TT; blocks: per group
 };
 
 __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int T) {
@@ -52,95 +52,197 @@ __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int T) {
     return n < 0 ? 0 : (n < T ? n : T);
 }
 
-template <int LN> struct Shape {
+// ------------------------------------------------------------------------------------------------- what the kernels share
+// A workgroup is two halves of NT threads.  The consumers own the states: a lane NS states of a channel, LN lanes a channel.  The
+// producers stage the tile behind the one the consumers are at (softplus, gates, conversion, once per channel and step) into the
+// other half of the buffers and finish the tile in front of it (sums over the lanes of a channel, outputs): a recurrence alone is a
+// chain of dependent operations that one wave per SIMD cannot fill, and the two kinds of waves fill each other's gaps.  One barrier
+// per tile; loads are a tile ahead of their use.
+template <int LN_, int NS_, bool EL = false> struct Shape {
+    static constexpr int LN = LN_, NS = NS_;
+    static constexpr bool ELEMENTS = EL;                    // load one by one: fewer than four channels, or states in no whole quads
+    static constexpr int NP = LN * NS;                      // states with their padding
     static constexpr int CH = LN <= 4 ? 64 : 256 / LN;      // channels of a workgroup
-    static constexpr int NT = CH * LN;                      // its threads
+    static constexpr int NT = CH * LN;                      // threads of either half
+    static constexpr int NW = NT / 64;
+    static constexpr int PL = LN > 8 ? 4 : LN;              // parts in which a sum over a channel's lanes is handed to the producers
     static constexpr int QR = CH / 4;                       // quads of channels per step
     static constexpr int ROWS = NT / QR < TT ? NT / QR : TT;
-    static constexpr int PASSES = TT / ROWS;                // of the workgroup over a tile's [TT][CH]
-    static constexpr int BPASSES = (TT * LN + NT - 1) / NT;  // over a tile's [TT][4 LN] of B and C
-    static constexpr int NP = 4 * LN;
+    static constexpr int PASSES = TT / ROWS;                // of the producers over a tile's [TT][CH]
+    static constexpr int QB = NP / 4;                       // quads of states per step
+    static constexpr int BPASSES = (TT * QB + NT - 1) / NT;  // over a tile's [TT][NP] of B and C
+    typedef __attribute__((ext_vector_type(NS_))) float Vec;   // the states of a lane
 };
 
-// Where a workgroup is: its group of channels, its first channel (of all), how many of CH exist.
-template <int LN> struct Place {
-    int g, d0, n, b, c;
-    __device__ __forceinline__ Place(const Scan& p) {
-        const int per = p.dim / p.groups, blk = blockIdx.x % p.blocks;
+// Where a workgroup is: its group of channels, its first channel (of all), how many of CH exist; its sequence, chunk and steps.
+template <typename S> struct Place {
+    int g, d0, n, b, c, begin, end, live, tiles, block;
+    bool ragged;                // groups of channels in no whole quads
+    __device__ __forceinline__ Place(const Scan& p, int chunk) {
+        const int per = p.dim / p.groups;
+        block = blockIdx.x % p.blocks;
         g = blockIdx.x / p.blocks;
-        d0 = g * per + blk * Shape<LN>::CH;
-        n = per - blk * Shape<LN>::CH;
-        n = n < Shape<LN>::CH ? n : Shape<LN>::CH;
-        c = blockIdx.y;
+        d0 = g * per + block * S::CH;
+        n = per - block * S::CH;
+        n = n < S::CH ? n : S::CH;
+        ragged = per & 3;
+        c = chunk;
         b = blockIdx.z;
+        const int len = length_of(p.lengths, b, p.T);
+        begin = c * p.chunk;
+        end = begin + p.chunk < p.T ? begin + p.chunk : p.T;
+        live = len < end ? len : end;
+        tiles = begin < live ? (live - begin + TT - 1) / TT : 0;
     }
 };
 
-// A [TT][CH] tile of one tensor in the registers of the threads that stage it: quad `q` of row pass * ROWS + row.
-template <typename T, int LN> struct Tile {
-    avsi_raw<T, 4> v[Shape<LN>::PASSES];
-    __device__ __forceinline__ void load(const void* base, int64_t bs, int64_t ts, const Place<LN>& at, int t0, int end) {
-        typedef Shape<LN> S;
-        const int q = threadIdx.x % S::QR, row = threadIdx.x / S::QR;
-        const T* p = (const T*)base + at.b * bs + at.d0 + 4 * q;
+// A producer's part of a tile: quad q of the channels, rows i * ROWS + row.
+// Nothing that loads may branch by lane (the join behind such a branch waits for the load): rows from `live` on read the last row, a
+// quad that goes over the last of all channels takes the last four and is shifted when it is used; what a group does not own is
+// masked where it is used.
+template <typename S> struct Stage {
+    int id, q, row, c;          // c: the channel (of all) at which the quad is loaded
+    bool on[4];                 // which of its channels exist
+    __device__ __forceinline__ Stage(const Scan& p, const Place<S>& at, int thread) {
+        id = thread;
+        q = id % S::QR, row = id / S::QR;
+        c = at.d0 + 4 * q;
+        if (!S::ELEMENTS) c = c < p.dim - 4 ? c : p.dim - 4;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) on[k] = 4 * q + k < at.n;
+    }
+    __device__ __forceinline__ bool stages() const { return 4 * S::LN <= TT || row < S::ROWS; }       // (wide states: some threads have no row)
+};
+// Row `i`'s place inside a tile that has `rows` rows left: 32 bits, on top of the tile's uniform address.
+__device__ __forceinline__ unsigned row_at(int i, int rows, int ts) { return (unsigned)((i < rows ? i : rows - 1) * ts); }
+
+template <typename T, typename S> struct Tile {
+    avsi_quad<T> v[S::PASSES];
+    __device__ __forceinline__ void load(const void* base, int64_t bs, int64_t ts, const Scan& p, const Place<S>& at, const Stage<S>& st, int t0) {
+        const T* b = (const T*)base + at.b * bs + t0 * ts;
 #pragma unroll
         for (int i = 0; i < S::PASSES; ++i) {
-            const int t = t0 + i * S::ROWS + row;
-            v[i] = avsi_load_raw<T, 4>(p + (int64_t)t * ts, row < S::ROWS && t < end ? at.n - 4 * q : 0);
+            const unsigned r = row_at(i * S::ROWS + st.row, at.live - t0, (int)ts);
+            if (!S::ELEMENTS) {
+                v[i].load(b + (r + st.c));
+            } else {
+                float f[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) f[k] = (float)b[r + (st.c + k < p.dim ? st.c + k : p.dim - 1)];
+                v[i].set(f);
+            }
+        }
+    }
+    __device__ __forceinline__ void get(int i, const Place<S>& at, const Stage<S>& st, float (&f)[4]) const {
+        v[i].get(f);
+        if (!S::ELEMENTS && at.ragged) {            // (a branch of the whole launch)
+            const int shift = at.d0 + 4 * st.q - st.c;
+            if (shift & 1) f[0] = f[1], f[1] = f[2], f[2] = f[3];
+            if (shift & 2) f[0] = f[2], f[1] = f[3];
         }
     }
 };
-template <typename T, int LN> struct TileBC {
-    avsi_raw<T, 4> v[Shape<LN>::BPASSES];
-    __device__ __forceinline__ void load(const void* base, int64_t bs, int64_t ts, int64_t gs, const Place<LN>& at, int N, int t0, int end) {
-        typedef Shape<LN> S;
+template <typename T, typename S> struct TileBC {
+    avsi_quad<T> v[S::BPASSES];
+    __device__ __forceinline__ void load(const void* base, int64_t bs, int64_t ts, int64_t gs, const Scan& p, const Place<S>& at,
+                                         const Stage<S>& st, int t0) {
+        const T* b = (const T*)base + at.b * bs + at.g * gs + t0 * ts;
 #pragma unroll
         for (int i = 0; i < S::BPASSES; ++i) {
-            const int id = i * S::NT + threadIdx.x, t = t0 + id / LN, n = 4 * (id % LN);
-            v[i] = avsi_load_raw<T, 4>((const T*)base + at.b * bs + at.g * gs + (int64_t)t * ts + n, id < TT * LN && t < end ? N - n : 0);
+            const int id = i * S::NT + st.id, n = 4 * (id % S::QB);
+            const unsigned r = row_at(id / S::QB % TT, at.live - t0, (int)ts);
+            if (!S::ELEMENTS) {
+                v[i].load(b + (r + (n < p.N ? n : p.N - 4)));
+            } else {
+                float f[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) f[k] = (float)b[r + (n + k < p.N ? n + k : p.N - 1)];
+                v[i].set(f);
+            }
         }
     }
-    __device__ __forceinline__ void put(avsi_f4* lds) const {       // [TT][LN]
-        typedef Shape<LN> S;
+    __device__ __forceinline__ void put(avsi_f4* lds, const Scan& p, const Place<S>& at, const Stage<S>& st, int t0) const {   // [TT][NP]
 #pragma unroll
         for (int i = 0; i < S::BPASSES; ++i) {
-            const int id = i * S::NT + threadIdx.x;
-            if (id < TT * LN) lds[id] = avsi_f4{(float)v[i].v[0], (float)v[i].v[1], (float)v[i].v[2], (float)v[i].v[3]};
+            const int id = i * S::NT + st.id, n = 4 * (id % S::QB);
+            float f[4];
+            v[i].get(f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = n + k < p.N && t0 + id / S::QB < at.live ? f[k] : 0.f;
+            if (S::BPASSES * S::NT == TT * S::QB || id < TT * S::QB) lds[id] = avsi_f4{f[0], f[1], f[2], f[3]};
         }
     }
 };
-
-__device__ __forceinline__ float step_size(float x, int softplus) { return softplus ? avsi_softplus(x) : x; }
-
-// dt_bias of this thread's quad of channels
-template <int LN> __device__ __forceinline__ void quad_of(const float* v, const Place<LN>& at, float other, float (&f)[4]) {
-    const int q = threadIdx.x % Shape<LN>::QR;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = v && 4 * q + i < at.n ? v[at.d0 + 4 * q + i] : other;
+template <typename T> __device__ __forceinline__ void put_quad(T* p, int n, const float (&f)[4]) {
+    avsi_quad<T> v;
+    v.set(f);
+    v.store(p, n);
 }
 
-// The four values of this lane in a [..][dim][NP] array at row d0 + channel; and A, times log2 e
-template <int LN> __device__ __forceinline__ int64_t lane_at(const Scan& p, const Place<LN>& at, int64_t lead) {
-    return ((lead * p.dim + at.d0 + threadIdx.x / LN) * LN + threadIdx.x % LN) * 4;
+// (both values and a choice: a branch, though one of the whole launch, would fence the schedule)
+__device__ __forceinline__ float step_size(float x, int softplus) {
+    const float s = avsi_softplus(x);
+    return softplus ? s : x;
 }
-template <int LN> __device__ __forceinline__ void lane_A(const Scan& p, const Place<LN>& at, float (&A)[4]) {
-    const int c = threadIdx.x / LN, n = 4 * (threadIdx.x % LN);
+
+// dt_bias, D of this thread's quad of channels
+template <typename S> __device__ __forceinline__ void quad_of(const float* v, const Place<S>& at, const Stage<S>& st, float (&f)[4]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) A[j] = c < at.n && n + j < p.N ? p.A[(int64_t)(at.d0 + c) * p.N + n + j] : 0.f;
+    for (int i = 0; i < 4; ++i) f[i] = v && st.on[i] ? v[at.d0 + 4 * st.q + i] : 0.f;
 }
-template <int LN> __device__ __forceinline__ void lane_start(const Scan& p, const Place<LN>& at, float (&h)[4]) {
-    const int c = threadIdx.x / LN, n = 4 * (threadIdx.x % LN);
+
+// A consumer's states in a [..][dim][NP] array at row `lead`, its A, and the state it starts from.
+template <typename S> __device__ __forceinline__ int64_t lane_at(const Scan& p, const Place<S>& at, int64_t lead) {
+    return ((lead * p.dim + at.d0 + threadIdx.x / S::LN) * S::LN + threadIdx.x % S::LN) * S::NS;
+}
+template <typename S> __device__ __forceinline__ void store_lane(float* p, const float (&f)[S::NS]) {
+    typename S::Vec v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = 0.f;
+    for (int j = 0; j < S::NS; ++j) v[j] = f[j];
+    *(typename S::Vec*)p = v;
+}
+template <typename S> __device__ __forceinline__ void lane_A(const Scan& p, const Place<S>& at, float (&A)[S::NS]) {
+    const int c = threadIdx.x / S::LN, n = S::NS * (threadIdx.x % S::LN);
+#pragma unroll
+    for (int j = 0; j < S::NS; ++j) A[j] = c < at.n && n + j < p.N ? p.A[(int64_t)(at.d0 + c) * p.N + n + j] : 0.f;
+}
+template <typename S> __device__ __forceinline__ void lane_start(const Scan& p, const Place<S>& at, float (&h)[S::NS]) {
+    const int c = threadIdx.x / S::LN, n = S::NS * (threadIdx.x % S::LN);
+#pragma unroll
+    for (int j = 0; j < S::NS; ++j) h[j] = 0.f;
     if (c >= at.n) return;
     if (at.c > 0) {
-        const avsi_f4 v = *(const avsi_f4*)(p.ends + lane_at<LN>(p, at, (int64_t)at.b * p.chunks + at.c));
+        const typename S::Vec v = *(const typename S::Vec*)(p.ends + lane_at<S>(p, at, (int64_t)at.b * p.chunks + at.c));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = v[j];
+        for (int j = 0; j < S::NS; ++j) h[j] = v[j];
     } else if (p.state) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < S::NS; ++j)
             if (n + j < p.N) h[j] = p.state[((int64_t)at.b * p.dim + at.d0 + c) * p.N + n + j];
+    }
+}
+
+// A sum over a channel's lanes: one value per lane into LDS, [channel][PL], and four channels' sums out of it.  Sixteen lanes hand
+// over four values (the buffers would not fit otherwise), the lanes that hold the same one all write it.
+template <typename S> __device__ __forceinline__ void put_part(avsi_f4* row, float v) {
+    if (S::LN == 16) {
+        v += avsi_dpp<0x128>(v);            // row_ror 8
+        v += avsi_dpp<0x124>(v);            // row_ror 4
+    }
+    ((float*)row)[threadIdx.x / S::LN * S::PL + threadIdx.x % S::PL] = v;
+}
+template <typename S> __device__ __forceinline__ void lane_sums(const avsi_f4* row, int q, float (&f)[4]) {
+    constexpr int PL = S::PL, V = PL < 4 ? PL : 4;
+    const float* p = (const float*)row + 4 * q * PL;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        f[k] = 0.f;
+#pragma unroll
+        for (int l = 0; l < PL; l += V) {
+            const avsi_raw<float, V> r = *(const avsi_raw<float, V>*)__builtin_assume_aligned(p + k * PL + l, 4 * V);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[k] += r.v[i];
+        }
     }
 }
 
@@ -148,179 +250,295 @@ template <int LN> __device__ __forceinline__ void lane_start(const Scan& p, cons
 __host__ __device__ __forceinline__ int64_t partial_stride(int dim, int NP) { return ((int64_t)dim * (NP + 2) + 3) / 4 * 4; }
 
 // ------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int LN> __global__ __launch_bounds__(Shape<LN>::NT) void scan_fwd_kernel(Scan p) {
-    typedef Shape<LN> S;
-    __shared__ avsi_f2 s_in[TT][S::CH];             // delta, delta u
-    __shared__ avsi_f4 s_B[TT * LN], s_C[TT * LN];
-    __shared__ float s_y[TT][S::CH];
-    const Place<LN> at(p);
-    const int len = length_of(p.lengths, at.b, p.T), begin = at.c * p.chunk;
-    const int end = begin + p.chunk < p.T ? begin + p.chunk : p.T, live = len < end ? len : end;
-    const int q = threadIdx.x % S::QR, row = threadIdx.x / S::QR, ch = threadIdx.x / LN, ql = threadIdx.x % LN;
-    float A[4], h[4], bias[4], Dq[4];
-    lane_A<LN>(p, at, A);
-    lane_start<LN>(p, at, h);
-    quad_of<LN>(p.bias, at, 0.f, bias);
-    quad_of<LN>(p.D, at, 0.f, Dq);
+// The consumers' decays are a group of two steps ahead of the states, and the operands of a group are read from LDS during the one
+// before; the fences keep the compiler from moving the reads back to their use.
+template <typename T, typename S> __global__ __launch_bounds__(2 * S::NT) void scan_fwd_kernel(Scan p) {
+    typedef typename S::Vec Vec;
+    __shared__ avsi_f2 s_in[2][TT][S::CH];             // delta, delta u
+    __shared__ avsi_f4 s_B[2][TT * S::QB], s_C[2][TT * S::QB];
+    __shared__ avsi_f4 s_y[2][TT][S::CH * S::PL / 4];          // C . h of each lane's states
+    const Place<S> at(p, blockIdx.y);
+    if (threadIdx.x < S::NT) {
+        const int ch = threadIdx.x / S::LN, ql = threadIdx.x % S::LN;
+        float A[S::NS], h[S::NS];
+        lane_A<S>(p, at, A);
+        lane_start<S>(p, at, h);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) A[j] *= LOG2E;
-    T* out = (T*)p.out + at.b * p.ob + at.d0 + 4 * q;
-    const int tiles = (p.T + TT - 1) / TT;
-
-    Tile<T, LN> u, dt, z;
-    TileBC<T, LN> Bt, Ct;
-    if (begin < live) {
-        u.load(p.u, p.ub, p.ut, at, begin, live);
-        dt.load(p.dt, p.tb, p.tt, at, begin, live);
-        if (p.z) z.load(p.z, p.zb, p.zt, at, begin, live);
-        Bt.load(p.B, p.Bb, p.Bt, p.Bg, at, p.N, begin, live);
-        Ct.load(p.C, p.Cb, p.Ct, p.Cg, at, p.N, begin, live);
-    }
-    int t0 = begin;
-    for (; t0 < live; t0 += TT) {
-        float through[S::PASSES][4], gate[S::PASSES][4];        // D u, and the gate
+        for (int j = 0; j < S::NS; ++j) A[j] *= LOG2E;
+        float* kept = p.kept && ch < at.n ? p.kept + lane_at<S>(p, at, (int64_t)at.b * ((p.T + TT - 1) / TT) + at.begin / TT) : nullptr;
+        AVSI_LDS_BARRIER();
+        for (int n = 0; n < at.tiles; ++n) {
+            const int buf = n & 1;
+            avsi_f2 in[TT];
 #pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            const int r = i * S::ROWS + row;
-            if (row < S::ROWS) {
+            for (int t = 0; t < TT; ++t) in[t] = s_in[buf][t][ch];
+            Vec Bv[2], Cv[2], Bn[2], Cn[2];
+            auto fetch = [&](int t) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float uf = (float)u.v[i].v[k];
-                    const float d = t0 + r < live ? step_size((float)dt.v[i].v[k] + bias[k], p.softplus) : 0.f;
-                    s_in[r][4 * q + k] = avsi_f2{d, d * uf};
-                    through[i][k] = Dq[k] * uf;
-                    const float zf = p.z ? (float)z.v[i].v[k] : 0.f;
-                    gate[i][k] = p.z ? zf * avsi_sigmoid(zf) : 1.f;
+                for (int j = 0; j < 2; ++j) {
+                    Bn[j] = ((const Vec*)s_B[buf])[(t + j) * S::LN + ql];
+                    Cn[j] = ((const Vec*)s_C[buf])[(t + j) * S::LN + ql];
                 }
-            }
-        }
-        Bt.put(s_B);
-        Ct.put(s_C);
-        AVSI_LDS_BARRIER();
-        if (p.kept && ch < at.n)
-            *(avsi_f4*)(p.kept + lane_at<LN>(p, at, (int64_t)at.b * tiles + t0 / TT)) = avsi_f4{h[0], h[1], h[2], h[3]};
-        if (t0 + TT < live) {
-            u.load(p.u, p.ub, p.ut, at, t0 + TT, live);
-            dt.load(p.dt, p.tb, p.tt, at, t0 + TT, live);
-            if (p.z) z.load(p.z, p.zb, p.zt, at, t0 + TT, live);
-            Bt.load(p.B, p.Bb, p.Bt, p.Bg, at, p.N, t0 + TT, live);
-            Ct.load(p.C, p.Cb, p.Ct, p.Cg, at, p.N, t0 + TT, live);
-        }
+            };
+            float a[2][S::NS], next[2][S::NS];
+            auto decays = [&](int t) {
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            const avsi_f2 in = s_in[t][ch];
-            const avsi_f4 Bv = s_B[t * LN + ql], Cv = s_C[t * LN + ql];
-            float y = 0.f;
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                h[j] = fmaf(__builtin_amdgcn_exp2f(in[0] * A[j]), h[j], in[1] * Bv[j]);
-                y = fmaf(h[j], Cv[j], y);
+                    for (int j = 0; j < S::NS; ++j) next[k][j] = __builtin_amdgcn_exp2f(in[t + k][0] * A[j]);
+            };
+            if (kept) store_lane<S>(kept + (int64_t)n * p.dim * S::NP, h);
+            fetch(0);
+            decays(0);
+#pragma unroll
+            for (int t = 0; t < TT; t += 2) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    Bv[k] = Bn[k], Cv[k] = Cn[k];
+#pragma unroll
+                    for (int j = 0; j < S::NS; ++j) a[k][j] = next[k][j];
+                }
+                if (t + 2 < TT) fetch(t + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                if (t + 2 < TT) decays(t + 2);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float y = 0.f;
+#pragma unroll
+                    for (int j = 0; j < S::NS; ++j) {
+                        h[j] = fmaf(a[k][j], h[j], in[t + k][1] * Bv[k][j]);
+                        y = fmaf(h[j], Cv[k][j], y);
+                    }
+                    put_part<S>(s_y[buf][t + k], y);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            y = avsi_group<LN>(y);
-            if (ql == t % LN) s_y[t][ch] = y;
+            AVSI_LDS_BARRIER();
         }
-        AVSI_LDS_BARRIER();
+        if (p.state_out && at.c == p.chunks - 1 && ch < at.n)
+#pragma unroll
+            for (int j = 0; j < S::NS; ++j)
+                if (S::NS * ql + j < p.N) p.state_out[((int64_t)at.b * p.dim + at.d0 + ch) * p.N + S::NS * ql + j] = h[j];
+        return;
+    }
+    const Stage<S> st(p, at, threadIdx.x - S::NT);
+    float bias[4], Dq[4];
+    quad_of<S>(p.bias, at, st, bias);
+    quad_of<S>(p.D, at, st, Dq);
+    T* out = (T*)p.out + at.b * p.ob + at.d0 + 4 * st.q;
+    Tile<T, S> u, dt, z;
+    TileBC<T, S> Bt, Ct;
+    auto load = [&](int n) {
+        const int t0 = at.begin + (n < at.tiles ? n : at.tiles - 1) * TT;
+        u.load(p.u, p.ub, p.ut, p, at, st, t0);
+        dt.load(p.dt, p.tb, p.tt, p, at, st, t0);
+        z.load(p.z, p.zb, p.zt, p, at, st, t0);
+        Bt.load(p.B, p.Bb, p.Bt, p.Bg, p, at, st, t0);
+        Ct.load(p.C, p.Cb, p.Ct, p.Cg, p, at, st, t0);
+    };
+    float thru[3][S::PASSES][4], gate[3][S::PASSES][4];         // D u and the gate, of the tiles n - 1, n and n + 1
+    auto stage = [&](int n) {
+        const int t0 = at.begin + n * TT, buf = n & 1;
+        float uf[S::PASSES][4], df[S::PASSES][4], zf[S::PASSES][4];
 #pragma unroll
         for (int i = 0; i < S::PASSES; ++i) {
-            const int t = t0 + i * S::ROWS + row;
-            if (row < S::ROWS && t < end) {
-                float o[4];
+            u.get(i, at, st, uf[i]);
+            dt.get(i, at, st, df[i]);
+            z.get(i, at, st, zf[i]);
+        }
+        Bt.put(s_B[buf], p, at, st, t0);
+        Ct.put(s_C[buf], p, at, st, t0);
+        load(n + 1);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    o[k] = t < live ? (s_y[i * S::ROWS + row][4 * q + k] + through[i][k]) * gate[i][k] : 0.f;
-                avsi_store<T, 4>(out + (int64_t)t * p.ot, at.n - 4 * q, o);
+        for (int i = 0; i < S::PASSES; ++i) {
+            float d[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool on = st.on[k] && t0 + i * S::ROWS + st.row < at.live;
+                const float s = step_size(df[i][k] + bias[k], p.softplus), g = zf[i][k] * avsi_sigmoid(zf[i][k]);
+                d[k] = on ? s : 0.f;
+                uf[i][k] = on ? uf[i][k] : 0.f;
+                thru[2][i][k] = Dq[k] * uf[i][k];
+                gate[2][i][k] = p.gated ? g : 1.f;
+            }
+            if (st.stages()) {
+                avsi_f4* to = (avsi_f4*)&s_in[buf][i * S::ROWS + st.row][4 * st.q];
+                to[0] = avsi_f4{d[0], d[0] * uf[i][0], d[1], d[1] * uf[i][1]};
+                to[1] = avsi_f4{d[2], d[2] * uf[i][2], d[3], d[3] * uf[i][3]};
             }
         }
-    }
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    if (row < S::ROWS)
-        for (int t = t0 + row; t < end; t += S::ROWS) avsi_store<T, 4>(out + (int64_t)t * p.ot, at.n - 4 * q, zero);
-    if (p.state_out && at.c == p.chunks - 1 && ch < at.n)
+    };
+    auto write = [&](int n) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (4 * ql + j < p.N) p.state_out[((int64_t)at.b * p.dim + at.d0 + ch) * p.N + 4 * ql + j] = h[j];
+        for (int i = 0; i < S::PASSES; ++i) {
+            const int r = i * S::ROWS + st.row, t = at.begin + n * TT + r;
+            if (st.stages() && t < at.end) {
+                float o[4];
+                lane_sums<S>(s_y[n & 1][r], st.q, o);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = t < at.live ? (o[k] + thru[0][i][k]) * gate[0][i][k] : 0.f;
+                put_quad<T>(out + (int64_t)t * p.ot, at.n - 4 * st.q, o);
+            }
+        }
+    };
+    auto turn = [&]() {
+#pragma unroll
+        for (int i = 0; i < S::PASSES; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                thru[0][i][k] = thru[1][i][k], thru[1][i][k] = thru[2][i][k];
+                gate[0][i][k] = gate[1][i][k], gate[1][i][k] = gate[2][i][k];
+            }
+    };
+    if (at.tiles) {
+        load(0);
+        stage(0);
+        turn();
+    }
+    AVSI_LDS_BARRIER();
+    for (int n = 0; n < at.tiles; ++n) {
+        if (n + 1 < at.tiles) stage(n + 1);
+        if (n > 0) write(n - 1);
+        turn();
+        AVSI_LDS_BARRIER();
+    }
+    if (at.tiles) write(at.tiles - 1);
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    if (st.stages())
+        for (int t = at.begin + at.tiles * TT + st.row; t < at.end; t += S::ROWS) put_quad<T>(out + (int64_t)t * p.ot, at.n - 4 * st.q, zero);
 }
 
 // A chunk from a zero state: its end state and the sum of its step sizes.  BACK: the adjoint state, from behind.
-template <typename T, int LN, bool BACK> __global__ __launch_bounds__(Shape<LN>::NT) void scan_chunk_kernel(Scan p) {
-    typedef Shape<LN> S;
-    __shared__ avsi_f2 s_in[TT][S::CH];             // delta, delta u (BACK: dy)
-    __shared__ avsi_f4 s_B[TT * LN];                // (BACK: C)
-    Place<LN> at(p);
-    if (BACK) ++at.c;                               // (the first chunk's is not needed; forward: the last one's)
-    const int len = length_of(p.lengths, at.b, p.T), begin = at.c * p.chunk;
-    const int end = begin + p.chunk < p.T ? begin + p.chunk : p.T, live = len < end ? len : end;
-    const int q = threadIdx.x % S::QR, row = threadIdx.x / S::QR, ch = threadIdx.x / LN, ql = threadIdx.x % LN;
-    float A[4], h[4] = {0.f, 0.f, 0.f, 0.f}, bias[4], sum = 0.f;
-    lane_A<LN>(p, at, A);
-    quad_of<LN>(p.bias, at, 0.f, bias);
+template <typename T, typename S, bool BACK> __global__ __launch_bounds__(2 * S::NT) void scan_chunk_kernel(Scan p) {
+    typedef typename S::Vec Vec;
+    __shared__ avsi_f2 s_in[2][TT][S::CH];             // delta, delta u (BACK: dy)
+    __shared__ avsi_f4 s_B[2][TT * S::QB];             // (BACK: C)
+    const Place<S> at(p, blockIdx.y + (BACK ? 1 : 0));  // (the first chunk's is not needed; forward: the last one's)
+    if (threadIdx.x < S::NT) {
+        const int ch = threadIdx.x / S::LN, ql = threadIdx.x % S::LN;
+        float A[S::NS], h[S::NS] = {}, sum = 0.f;
+        lane_A<S>(p, at, A);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) A[j] *= LOG2E;
-    const int n_tiles = begin < live ? (live - begin + TT - 1) / TT : 0;
-    Tile<T, LN> u, dt, z;                           // BACK: u is dout
-    TileBC<T, LN> Bt;
-    auto load = [&](int t0) {
-        dt.load(p.dt, p.tb, p.tt, at, t0, live);
+        for (int j = 0; j < S::NS; ++j) A[j] *= LOG2E;
+        AVSI_LDS_BARRIER();
+        for (int n = 0; n < at.tiles; ++n) {
+            const int buf = n & 1;
+            avsi_f2 in[TT];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) in[t] = s_in[buf][BACK ? TT - 1 - t : t][ch];
+            Vec Bv[2], Bn[2];
+            auto fetch = [&](int t) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) Bn[j] = ((const Vec*)s_B[buf])[(BACK ? TT - 1 - t - j : t + j) * S::LN + ql];
+            };
+            float a[2][S::NS], next[2][S::NS];
+            auto decays = [&](int t) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int j = 0; j < S::NS; ++j) next[k][j] = __builtin_amdgcn_exp2f(in[t + k][0] * A[j]);
+            };
+            fetch(0);
+            decays(0);
+            float part = 0.f;               // (a tile's own sum: the long one keeps its low bits)
+#pragma unroll
+            for (int t = 0; t < TT; t += 2) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    Bv[k] = Bn[k];
+#pragma unroll
+                    for (int j = 0; j < S::NS; ++j) a[k][j] = next[k][j];
+                }
+                if (t + 2 < TT) fetch(t + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                if (t + 2 < TT) decays(t + 2);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    part += in[t + k][0];
+#pragma unroll
+                    for (int j = 0; j < S::NS; ++j)
+                        h[j] = BACK ? a[k][j] * fmaf(Bv[k][j], in[t + k][1], h[j]) : fmaf(a[k][j], h[j], in[t + k][1] * Bv[k][j]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            sum += part;
+            AVSI_LDS_BARRIER();
+        }
+        if (ch < at.n) {
+            // the chunk's row of `ends` is read as the start of the chunk behind it (in front of it)
+            const int64_t lead = (int64_t)at.b * p.chunks + (BACK ? at.c - 1 : at.c + 1);
+            store_lane<S>(p.ends + lane_at<S>(p, at, lead), h);
+            if (ql == 0) p.sums[lead * p.dim + at.d0 + ch] = sum;
+        }
+        return;
+    }
+    const Stage<S> st(p, at, threadIdx.x - S::NT);
+    float bias[4];
+    quad_of<S>(p.bias, at, st, bias);
+    Tile<T, S> u, dt, z;                               // BACK: u is dout
+    TileBC<T, S> Bt;
+    auto tile_at = [&](int n) { return at.begin + (BACK ? at.tiles - 1 - n : n) * TT; };
+    auto load = [&](int n) {
+        const int t0 = tile_at(n < at.tiles ? n : at.tiles - 1);
+        dt.load(p.dt, p.tb, p.tt, p, at, st, t0);
         if (BACK) {
-            u.load(p.dout, p.gb, p.gt, at, t0, live);
-            if (p.z) z.load(p.z, p.zb, p.zt, at, t0, live);
-            Bt.load(p.C, p.Cb, p.Ct, p.Cg, at, p.N, t0, live);
+            u.load(p.dout, p.gb, p.gt, p, at, st, t0);
+            z.load(p.z, p.zb, p.zt, p, at, st, t0);
+            Bt.load(p.C, p.Cb, p.Ct, p.Cg, p, at, st, t0);
         } else {
-            u.load(p.u, p.ub, p.ut, at, t0, live);
-            Bt.load(p.B, p.Bb, p.Bt, p.Bg, at, p.N, t0, live);
+            u.load(p.u, p.ub, p.ut, p, at, st, t0);
+            Bt.load(p.B, p.Bb, p.Bt, p.Bg, p, at, st, t0);
         }
     };
-    auto tile_at = [&](int i) { return begin + (BACK ? n_tiles - 1 - i : i) * TT; };
-    if (n_tiles) load(tile_at(0));
-    for (int i = 0; i < n_tiles; ++i) {
-        const int t0 = tile_at(i);
+    auto stage = [&](int n) {
+        const int t0 = tile_at(n), buf = n & 1;
+        float x[S::PASSES][4], df[S::PASSES][4], zf[S::PASSES][4];
 #pragma unroll
-        for (int k = 0; k < S::PASSES; ++k) {
-            const int r = k * S::ROWS + row;
-            if (row < S::ROWS) {
+        for (int i = 0; i < S::PASSES; ++i) {
+            u.get(i, at, st, x[i]);
+            dt.get(i, at, st, df[i]);
+            if (BACK) z.get(i, at, st, zf[i]);
+        }
+        Bt.put(s_B[buf], p, at, st, t0);
+        load(n + 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float d = t0 + r < live ? step_size((float)dt.v[k].v[j] + bias[j], p.softplus) : 0.f;
-                    float x = (float)u.v[k].v[j];
-                    if (BACK) {
-                        if (p.z) x *= (float)z.v[k].v[j] * avsi_sigmoid((float)z.v[k].v[j]);
-                    } else {
-                        x *= d;
-                    }
-                    s_in[r][4 * q + j] = avsi_f2{d, x};
+        for (int i = 0; i < S::PASSES; ++i) {
+            float d[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool on = st.on[k] && t0 + i * S::ROWS + st.row < at.live;
+                const float s = step_size(df[i][k] + bias[k], p.softplus);
+                d[k] = on ? s : 0.f;
+                if (BACK) {
+                    const float gate = zf[i][k] * avsi_sigmoid(zf[i][k]);
+                    x[i][k] = on ? x[i][k] * (p.gated ? gate : 1.f) : 0.f;
+                } else {
+                    x[i][k] = on ? x[i][k] * s : 0.f;
                 }
             }
-        }
-        Bt.put(s_B);
-        AVSI_LDS_BARRIER();
-        if (i + 1 < n_tiles) load(tile_at(i + 1));
-#pragma unroll
-        for (int k = 0; k < TT; ++k) {
-            const int t = BACK ? TT - 1 - k : k;
-            const avsi_f2 in = s_in[t][ch];
-            const avsi_f4 Bv = s_B[t * LN + ql];
-            sum += in[0];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float a = __builtin_amdgcn_exp2f(in[0] * A[j]);
-                h[j] = BACK ? a * fmaf(Bv[j], in[1], h[j]) : fmaf(a, h[j], in[1] * Bv[j]);
+            if (st.stages()) {
+                avsi_f4* to = (avsi_f4*)&s_in[buf][i * S::ROWS + st.row][4 * st.q];
+                to[0] = avsi_f4{d[0], x[i][0], d[1], x[i][1]};
+                to[1] = avsi_f4{d[2], x[i][2], d[3], x[i][3]};
             }
         }
-        AVSI_LDS_BARRIER();
+    };
+    if (at.tiles) {
+        load(0);
+        stage(0);
     }
-    if (ch < at.n) {
-        // the chunk's row of `ends` is read as the start of the chunk behind it (in front of it)
-        const int64_t lead = (int64_t)at.b * p.chunks + (BACK ? at.c - 1 : at.c + 1);
-        *(avsi_f4*)(p.ends + lane_at<LN>(p, at, lead)) = avsi_f4{h[0], h[1], h[2], h[3]};
-        if (ql == 0) p.sums[lead * p.dim + at.d0 + ch] = sum;
+    AVSI_LDS_BARRIER();
+    for (int n = 0; n < at.tiles; ++n) {
+        if (n + 1 < at.tiles) stage(n + 1);
+        AVSI_LDS_BARRIER();
     }
 }
 
 // start[c] = local end of c - 1 + exp(A sum of c - 1) start[c - 1] (BACK: with c + 1), in place.  One thread per four states.
-template <int LN, bool BACK> __global__ __launch_bounds__(256) void scan_join_kernel(Scan p) {
+template <bool BACK> __global__ __launch_bounds__(256) void scan_join_kernel(Scan p, int QB) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= (int64_t)p.batch * p.dim * LN) return;
-    const int ql = (int)(id % LN), d = (int)(id / LN % p.dim), b = (int)(id / LN / p.dim);
+    if (id >= (int64_t)p.batch * p.dim * QB) return;
+    const int ql = (int)(id % QB), d = (int)(id / QB % p.dim), b = (int)(id / QB / p.dim);
     float A[4], h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -330,7 +548,7 @@ template <int LN, bool BACK> __global__ __launch_bounds__(256) void scan_join_ke
     }
     for (int i = 1; i < p.chunks; ++i) {
         const int64_t lead = (int64_t)b * p.chunks + (BACK ? p.chunks - 1 - i : i);
-        avsi_f4* e = (avsi_f4*)(p.ends + ((lead * p.dim + d) * LN + ql) * 4);
+        avsi_f4* e = (avsi_f4*)(p.ends + ((lead * p.dim + d) * QB + ql) * 4);
         const float s = p.sums[lead * p.dim + d];
         avsi_f4 v = *e;
 #pragma unroll
@@ -340,201 +558,262 @@ template <int LN, bool BACK> __global__ __launch_bounds__(256) void scan_join_ke
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
-// Sum over the channels of a wave (the lanes that share a quad of states) of b[0 .. 3] and c[0 .. 3], at *out = [2][NP] of one step.
-// While a level halves the lanes it halves the values too: the upper half of the lanes takes c, then the odd rows values 2 and 3.
-template <int LN> __device__ __forceinline__ void channel_sums(float (&b)[4], float (&c)[4], float* out) {
-    const int lane = threadIdx.x & 63, q = lane % LN;
+// Sum over the channels of a wave (the lanes that share a place among the states) of b and c, at *out = [2][NP] of one step.
+// While a level halves the lanes it halves the values too: the upper half of the lanes takes c, then the odd rows the upper states.
+template <typename S> __device__ __forceinline__ void channel_sums(float (&b)[S::NS], float (&c)[S::NS], float* out) {
+    constexpr int LN = S::LN, H = S::NS / 2;
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < S::NS; ++j) {
         avsi_swap32(b[j], c[j]);
         b[j] += c[j];
     }
-    float* o = out + (lane >> 5) * 4 * LN + 4 * q;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        avsi_swap16(b[j], b[j + 2]);
-        b[j] += b[j + 2];
+    for (int j = 0; j < H; ++j) {
+        avsi_swap16(b[j], b[j + H]);
+        b[j] += b[j + H];
         if (LN <= 8) b[j] += avsi_dpp<0x128>(b[j]);         // row_ror 8
         if (LN <= 4) b[j] += avsi_dpp<0x124>(b[j]);         // row_ror 4
         if (LN <= 2) b[j] += avsi_dpp<0x4E>(b[j]);
         if (LN <= 1) b[j] += avsi_dpp<0xB1>(b[j]);
     }
-    if ((lane & 15) < LN) {
-        o += ((lane >> 4) & 1) * 2;
-        o[0] = b[0];
-        o[1] = b[1];
-    }
+    // (the lanes of a row that hold the same sums all write them: a branch here would fence the schedule of every step)
+    float* o = out + (lane >> 5) * S::NP + S::NS * (lane % LN) + ((lane >> 4) & 1) * H;
+#pragma unroll
+    for (int j = 0; j < H; ++j) o[j] = b[j];
 }
 
-template <typename T, int LN> __global__ __launch_bounds__(Shape<LN>::NT) void scan_bwd_kernel(Scan p) {
-    typedef Shape<LN> S;
-    constexpr int NW = S::NT / 64;
-    __shared__ avsi_f4 s_in[TT][S::CH];             // delta, delta u, dy
-    __shared__ avsi_f4 s_B[TT * LN], s_C[TT * LN];
-    __shared__ float s_y[TT][S::CH], s_gB[TT][S::CH], s_gA[TT][S::CH];
-    __shared__ float s_bc[NW][TT][2 * S::NP];
-    const Place<LN> at(p);
-    const int len = length_of(p.lengths, at.b, p.T), begin = at.c * p.chunk;
-    const int end = begin + p.chunk < p.T ? begin + p.chunk : p.T, live = len < end ? len : end;
-    const int q = threadIdx.x % S::QR, row = threadIdx.x / S::QR, ch = threadIdx.x / LN, ql = threadIdx.x % LN;
-    float A[4], Al[4], g[4] = {0.f, 0.f, 0.f, 0.f}, dA[4] = {0.f, 0.f, 0.f, 0.f}, bias[4], Dq[4], dD[4], dbias[4];
-    lane_A<LN>(p, at, A);
-    quad_of<LN>(p.bias, at, 0.f, bias);
-    quad_of<LN>(p.D, at, 0.f, Dq);
+// A tile is 16 steps forward from its kept state, decays and states staying in the registers of the consumers, and 16 steps back
+// over them.
+template <typename T, typename S> __global__ __launch_bounds__(2 * S::NT) void scan_bwd_kernel(Scan p) {
+    typedef typename S::Vec Vec;
+    __shared__ avsi_f4 s_in[2][TT][S::CH];             // delta, delta u, dy
+    __shared__ avsi_f4 s_B[2][TT * S::QB], s_C[2][TT * S::QB];
+    __shared__ avsi_f4 s_y[2][TT][S::CH * S::PL / 4], s_gB[2][TT][S::CH * S::PL / 4], s_gA[2][TT][S::CH * S::PL / 4];      // sums over each lane's states
+    __shared__ float s_bc[2][S::NW][TT][2 * S::NP];
+    const Place<S> at(p, blockIdx.y);
+    auto tile_at = [&](int n) { return at.begin + (at.tiles - 1 - n) * TT; };
+    float* pw = p.part_w + ((int64_t)at.b * p.chunks + at.c) * partial_stride(p.dim, S::NP);
+    if (threadIdx.x < S::NT) {
+        const int ch = threadIdx.x / S::LN, ql = threadIdx.x % S::LN;
+        float A[S::NS], Al[S::NS], g[S::NS] = {}, dA[S::NS] = {};
+        lane_A<S>(p, at, A);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        Al[j] = A[j] * LOG2E;
-        dD[j] = dbias[j] = 0.f;
-    }
-    if (at.c < p.chunks - 1 && ch < at.n) {
-        const avsi_f4 v = *(const avsi_f4*)(p.ends + lane_at<LN>(p, at, (int64_t)at.b * p.chunks + at.c));
+        for (int j = 0; j < S::NS; ++j) Al[j] = A[j] * LOG2E;
+        if (at.c < p.chunks - 1 && ch < at.n) {
+            const Vec v = *(const Vec*)(p.ends + lane_at<S>(p, at, (int64_t)at.b * p.chunks + at.c));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) g[j] = v[j];
-    }
-    const int tiles = (p.T + TT - 1) / TT, n_tiles = begin < live ? (live - begin + TT - 1) / TT : 0;
-    const int64_t flat = ((int64_t)at.b * p.T) * p.dim + at.d0 + 4 * q;
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    if (row < S::ROWS)
-        for (int t = begin + n_tiles * TT + row; t < end; t += S::ROWS) {
-            avsi_store<T, 4>((T*)p.du + flat + (int64_t)t * p.dim, at.n - 4 * q, zero);
-            avsi_store<T, 4>((T*)p.ddt + flat + (int64_t)t * p.dim, at.n - 4 * q, zero);
-            if (p.z) avsi_store<T, 4>((T*)p.dz + flat + (int64_t)t * p.dim, at.n - 4 * q, zero);
+            for (int j = 0; j < S::NS; ++j) g[j] = v[j];
         }
-    Tile<T, LN> u, dt, z, go;
-    TileBC<T, LN> Bt, Ct;
-    avsi_f4 start = {0.f, 0.f, 0.f, 0.f};
-    auto load = [&](int t0) {
-        u.load(p.u, p.ub, p.ut, at, t0, live);
-        dt.load(p.dt, p.tb, p.tt, at, t0, live);
-        go.load(p.dout, p.gb, p.gt, at, t0, live);
-        if (p.z) z.load(p.z, p.zb, p.zt, at, t0, live);
-        Bt.load(p.B, p.Bb, p.Bt, p.Bg, at, p.N, t0, live);
-        Ct.load(p.C, p.Cb, p.Ct, p.Cg, at, p.N, t0, live);
-        if (ch < at.n) start = *(const avsi_f4*)(p.kept + lane_at<LN>(p, at, (int64_t)at.b * tiles + t0 / TT));
+        // (lanes without a channel read the last one's)
+        const float* kept = p.kept + lane_at<S>(p, at, (int64_t)at.b * ((p.T + TT - 1) / TT)) - (ch < at.n ? 0 : (int64_t)(ch - at.n + 1) * S::NP);
+        Vec start;
+        auto load = [&](int n) { start = *(const Vec*)(kept + (int64_t)(tile_at(n < at.tiles ? n : at.tiles - 1) / TT) * p.dim * S::NP); };
+        if (at.tiles) load(0);
+        AVSI_LDS_BARRIER();
+        for (int n = 0; n < at.tiles; ++n) {
+            const int buf = n & 1;
+            float h[S::NS];
+#pragma unroll
+            for (int j = 0; j < S::NS; ++j) h[j] = start[j];
+            load(n + 1);
+            float a[TT][S::NS], before[TT][S::NS];
+            avsi_f4 in[2], in2[2];
+            Vec Bv[2], Cv[2], Bn[2], Cn[2];
+            auto fetch = [&](int t) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    in2[j] = s_in[buf][t + j][ch];
+                    Bn[j] = ((const Vec*)s_B[buf])[(t + j) * S::LN + ql];
+                    Cn[j] = ((const Vec*)s_C[buf])[(t + j) * S::LN + ql];
+                }
+            };
+            auto take = [&]() {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) in[j] = in2[j], Bv[j] = Bn[j], Cv[j] = Cn[j];
+            };
+            fetch(0);
+#pragma unroll
+            for (int t = 0; t < TT; t += 2) {
+                take();
+                fetch(t + 2 < TT ? t + 2 : TT - 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float y = 0.f;                          // (for dz; without a gate it is not read)
+#pragma unroll
+                    for (int j = 0; j < S::NS; ++j) {
+                        before[t + k][j] = h[j];
+                        a[t + k][j] = __builtin_amdgcn_exp2f(in[k][0] * Al[j]);
+                        h[j] = fmaf(a[t + k][j], h[j], in[k][1] * Bv[k][j]);
+                        y = fmaf(h[j], Cv[k][j], y);
+                    }
+                    put_part<S>(s_y[buf][t + k], y);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float dAt[S::NS] = {};        // (a tile's own sum: the long sum over time keeps its low bits)
+#pragma unroll
+            for (int t2 = TT - 2; t2 >= 0; t2 -= 2) {
+                take();
+                if (t2 > 0) fetch(t2 - 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 1; k >= 0; --k) {
+                    const int t = t2 + k;
+                    float vb[S::NS], vc[S::NS], gB = 0.f, gA = 0.f;
+#pragma unroll
+                    for (int j = 0; j < S::NS; ++j) {
+                        const float gj = fmaf(Cv[k][j], in[k][2], g[j]);
+                        vb[j] = gj * in[k][1];
+                        vc[j] = in[k][2] * (t == TT - 1 ? h[j] : before[t == TT - 1 ? t : t + 1][j]);
+                        gB = fmaf(gj, Bv[k][j], gB);
+                        g[j] = a[t][j] * gj;
+                        const float x = g[j] * before[t][j];
+                        gA = fmaf(x, A[j], gA);
+                        dAt[j] = fmaf(x, in[k][0], dAt[j]);
+                    }
+                    put_part<S>(s_gB[buf][t], gB);
+                    put_part<S>(s_gA[buf][t], gA);
+                    channel_sums<S>(vb, vc, s_bc[buf][threadIdx.x >> 6][t]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int j = 0; j < S::NS; ++j) dA[j] += dAt[j];
+            AVSI_LDS_BARRIER();
+        }
+        if (ch < at.n) store_lane<S>(pw + ((int64_t)(at.d0 + ch) * S::LN + ql) * S::NS, dA);
+        AVSI_LDS_BARRIER();
+        AVSI_LDS_BARRIER();
+        return;
+    }
+    const Stage<S> st(p, at, threadIdx.x - S::NT);
+    float bias[4], Dq[4], dD[4] = {}, dbias[4] = {};
+    quad_of<S>(p.bias, at, st, bias);
+    quad_of<S>(p.D, at, st, Dq);
+    const int64_t flat = (int64_t)at.b * p.T * p.dim + at.d0 + 4 * st.q;
+    const int left = at.n - 4 * st.q;
+    auto put = [&](int t, const float (&du)[4], const float (&ddt)[4], const float (&dz)[4]) {
+        const int64_t i = flat + (int64_t)t * p.dim;
+        put_quad<T>((T*)p.du + i, left, du);
+        put_quad<T>((T*)p.ddt + i, left, ddt);
+        if (p.gated) put_quad<T>((T*)p.dz + i, left, dz);
     };
-    if (n_tiles) load(begin + (n_tiles - 1) * TT);
-    for (int t0 = begin + (n_tiles - 1) * TT; t0 >= begin; t0 -= TT) {
-        float uf[S::PASSES][4], delta[S::PASSES][4], slope[S::PASSES][4], dy[S::PASSES][4], gz[S::PASSES][4];
+    Tile<T, S> u, dt, z, go;
+    TileBC<T, S> Bt, Ct;
+    auto load = [&](int n) {
+        const int t0 = tile_at(n < at.tiles ? n : at.tiles - 1);
+        u.load(p.u, p.ub, p.ut, p, at, st, t0);
+        dt.load(p.dt, p.tb, p.tt, p, at, st, t0);
+        go.load(p.dout, p.gb, p.gt, p, at, st, t0);
+        z.load(p.z, p.zb, p.zt, p, at, st, t0);
+        Bt.load(p.B, p.Bb, p.Bt, p.Bg, p, at, st, t0);
+        Ct.load(p.C, p.Cb, p.Ct, p.Cg, p, at, st, t0);
+    };
+    struct Held {                // what a tile's gradients need besides the consumers' sums
+        float u[4], delta[4], slope[4], dy[4], gz[4];
+    } held[3][S::PASSES];        // of the tiles n - 1, n and n + 1
+    auto stage = [&](int n) {
+        const int t0 = tile_at(n), buf = n & 1;
+        float df[S::PASSES][4], zf[S::PASSES][4], of[S::PASSES][4];
 #pragma unroll
         for (int i = 0; i < S::PASSES; ++i) {
-            const int r = i * S::ROWS + row;
-            if (row < S::ROWS) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float x = (float)dt.v[i].v[k] + bias[k];
-                    const bool on = t0 + r < live;
-                    uf[i][k] = (float)u.v[i].v[k];
-                    delta[i][k] = on ? step_size(x, p.softplus) : 0.f;
-                    slope[i][k] = on ? (p.softplus ? avsi_sigmoid(x) : 1.f) : 0.f;
-                    dy[i][k] = (float)go.v[i].v[k];
-                    if (p.z) {
-                        const float zf = (float)z.v[i].v[k], s = avsi_sigmoid(zf);
-                        gz[i][k] = dy[i][k] * s * fmaf(zf, 1.f - s, 1.f);
-                        dy[i][k] *= zf * s;
-                    }
-                    s_in[r][4 * q + k] = avsi_f4{delta[i][k], delta[i][k] * uf[i][k], dy[i][k], 0.f};
-                }
-            }
+            u.get(i, at, st, held[2][i].u);
+            dt.get(i, at, st, df[i]);
+            z.get(i, at, st, zf[i]);
+            go.get(i, at, st, of[i]);
         }
-        Bt.put(s_B);
-        Ct.put(s_C);
-        float h[4] = {start[0], start[1], start[2], start[3]};
-        AVSI_LDS_BARRIER();
-        if (t0 > begin) load(t0 - TT);
-        float a[TT][4], before[TT][4];
+        Bt.put(s_B[buf], p, at, st, t0);
+        Ct.put(s_C[buf], p, at, st, t0);
+        load(n + 1);
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            const avsi_f4 in = s_in[t][ch], Bv = s_B[t * LN + ql];
-            float y = 0.f;
+        for (int i = 0; i < S::PASSES; ++i) {
+            Held& w = held[2][i];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                before[t][j] = h[j];
-                a[t][j] = __builtin_amdgcn_exp2f(in[0] * Al[j]);
-                h[j] = fmaf(a[t][j], h[j], in[1] * Bv[j]);
+            for (int k = 0; k < 4; ++k) {
+                const bool on = st.on[k] && t0 + i * S::ROWS + st.row < at.live;
+                const float x = df[i][k] + bias[k], d = step_size(x, p.softplus), s = avsi_sigmoid(x), e = avsi_sigmoid(zf[i][k]);
+                w.u[k] = on ? w.u[k] : 0.f;
+                w.delta[k] = on ? d : 0.f;
+                w.slope[k] = on ? (p.softplus ? s : 1.f) : 0.f;
+                w.dy[k] = on ? of[i][k] * (p.gated ? zf[i][k] * e : 1.f) : 0.f;
+                w.gz[k] = on ? of[i][k] * (e * fmaf(zf[i][k], 1.f - e, 1.f)) : 0.f;
             }
-            if (p.z) {
-                const avsi_f4 Cv = s_C[t * LN + ql];
+            if (st.stages())
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y = fmaf(h[j], Cv[j], y);
-                y = avsi_group<LN>(y);
-                if (ql == t % LN) s_y[t][ch] = y;
-            }
+                for (int k = 0; k < 4; ++k)
+                    s_in[buf][i * S::ROWS + st.row][4 * st.q + k] = avsi_f4{w.delta[k], w.delta[k] * w.u[k], w.dy[k], 0.f};
         }
-        float dAt[4] = {0.f, 0.f, 0.f, 0.f};        // (a tile's own sum: the long sum over time keeps its low bits)
-#pragma unroll
-        for (int t = TT - 1; t >= 0; --t) {
-            const avsi_f4 in = s_in[t][ch], Bv = s_B[t * LN + ql], Cv = s_C[t * LN + ql];
-            float vb[4], vc[4], gB = 0.f, gA = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float gj = fmaf(Cv[j], in[2], g[j]);
-                vb[j] = gj * in[1];
-                vc[j] = in[2] * (t == TT - 1 ? h[j] : before[t == TT - 1 ? t : t + 1][j]);
-                gB = fmaf(gj, Bv[j], gB);
-                g[j] = a[t][j] * gj;
-                const float x = g[j] * before[t][j];
-                gA = fmaf(x, A[j], gA);
-                dAt[j] = fmaf(x, in[0], dAt[j]);
-            }
-            gB = avsi_group<LN>(gB);
-            gA = avsi_group<LN>(gA);
-            if (ql == t % LN) {
-                s_gB[t][ch] = gB;
-                s_gA[t][ch] = gA;
-            }
-            channel_sums<LN>(vb, vc, s_bc[threadIdx.x >> 6][t]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dA[j] += dAt[j];
-        AVSI_LDS_BARRIER();
-        for (int i = threadIdx.x; i < TT * 2 * S::NP; i += S::NT) {
+    };
+    auto finish = [&](int n) {
+        const int t0 = tile_at(n), buf = n & 1;
+        for (int i = st.id; i < TT * 2 * S::NP; i += S::NT) {
             float s = 0.f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) s += s_bc[w][i / (2 * S::NP)][i % (2 * S::NP)];
+            for (int w = 0; w < S::NW; ++w) s += s_bc[buf][w][i / (2 * S::NP)][i % (2 * S::NP)];
             const int t = t0 + i / (2 * S::NP);
-            if (t < live)
-                p.part_bc[((((int64_t)at.b * p.T + t) * p.groups + at.g) * p.blocks + blockIdx.x % p.blocks) * 2 * S::NP + i % (2 * S::NP)] = s;
+            if (t < at.live)
+                p.part_bc[((((int64_t)at.b * p.T + t) * p.groups + at.g) * p.blocks + at.block) * 2 * S::NP + i % (2 * S::NP)] = s;
         }
 #pragma unroll
         for (int i = 0; i < S::PASSES; ++i) {
-            const int r = i * S::ROWS + row, t = t0 + r;
-            if (row < S::ROWS && t < end) {
-                float o[4], od[4], oz[4];
+            const int r = i * S::ROWS + st.row, t = t0 + r;
+            if (st.stages() && t < at.end) {
+                const Held& w = held[0][i];
+                float du[4], ddt[4], dz[4], gB[4], gA[4], y[4];
+                lane_sums<S>(s_gB[buf][r], st.q, gB);
+                lane_sums<S>(s_gA[buf][r], st.q, gA);
+                lane_sums<S>(s_y[buf][r], st.q, y);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float gB = s_gB[r][4 * q + k];
-                    const bool on = t < live;
-                    o[k] = on ? fmaf(Dq[k], dy[i][k], delta[i][k] * gB) : 0.f;
-                    od[k] = on ? fmaf(uf[i][k], gB, s_gA[r][4 * q + k]) * slope[i][k] : 0.f;
-                    dD[k] = fmaf(dy[i][k], uf[i][k], dD[k]);
-                    dbias[k] += od[k];
-                    oz[k] = on && p.z ? gz[i][k] * fmaf(Dq[k], uf[i][k], s_y[r][4 * q + k]) : 0.f;
+                for (int k = 0; k < 4; ++k) {           // (behind a length everything held is zero)
+                    du[k] = fmaf(Dq[k], w.dy[k], w.delta[k] * gB[k]);
+                    ddt[k] = fmaf(w.u[k], gB[k], gA[k]) * w.slope[k];
+                    dz[k] = w.gz[k] * fmaf(Dq[k], w.u[k], y[k]);
+                    dD[k] = fmaf(w.dy[k], w.u[k], dD[k]);
+                    dbias[k] += ddt[k];
+                    if (t >= at.live) du[k] = ddt[k] = dz[k] = 0.f;
                 }
-                const int64_t o_at = flat + (int64_t)t * p.dim;
-                avsi_store<T, 4>((T*)p.du + o_at, at.n - 4 * q, o);
-                avsi_store<T, 4>((T*)p.ddt + o_at, at.n - 4 * q, od);
-                if (p.z) avsi_store<T, 4>((T*)p.dz + o_at, at.n - 4 * q, oz);
+                put(t, du, ddt, dz);
             }
         }
+    };
+    auto turn = [&]() {
+#pragma unroll
+        for (int i = 0; i < S::PASSES; ++i) held[0][i] = held[1][i], held[1][i] = held[2][i];
+    };
+    if (at.tiles) {
+        load(0);
+        stage(0);
+        turn();
     }
-    // the weights' gradients of this workgroup's channels, over its chunk
-    float* pw = p.part_w + ((int64_t)at.b * p.chunks + at.c) * partial_stride(p.dim, S::NP);
-    if (ch < at.n) *(avsi_f4*)(pw + ((int64_t)(at.d0 + ch) * LN + ql) * 4) = avsi_f4{dA[0], dA[1], dA[2], dA[3]};
     AVSI_LDS_BARRIER();
-    if (row < S::ROWS)
+    for (int n = 0; n < at.tiles; ++n) {
+        if (n + 1 < at.tiles) stage(n + 1);
+        if (n > 0) finish(n - 1);
+        turn();
+        AVSI_LDS_BARRIER();
+    }
+    if (at.tiles) finish(at.tiles - 1);
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    if (st.stages())
+        for (int t = at.begin + at.tiles * TT + st.row; t < at.end; t += S::ROWS) put(t, zero, zero, zero);
+    // D's and the bias' gradients of this workgroup's channels, over its chunk: the rows of the producers
+    AVSI_LDS_BARRIER();
+    if (st.stages())
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            s_gB[row][4 * q + k] = dD[k];
-            s_gA[row][4 * q + k] = dbias[k];
+            ((float*)s_gB[0][st.row])[4 * st.q + k] = dD[k];
+            ((float*)s_gA[0][st.row])[4 * st.q + k] = dbias[k];
         }
     AVSI_LDS_BARRIER();
-    if (threadIdx.x < at.n) {
+    if (st.id < at.n) {
         float sD = 0.f, sb = 0.f;
         for (int r = 0; r < S::ROWS; ++r) {
-            sD += s_gB[r][threadIdx.x];
-            sb += s_gA[r][threadIdx.x];
+            sD += ((const float*)s_gB[0][r])[st.id];
+            sb += ((const float*)s_gA[0][r])[st.id];
         }
-        pw += (int64_t)p.dim * S::NP + at.d0 + threadIdx.x;
+        pw += (int64_t)p.dim * S::NP + at.d0 + st.id;
         pw[0] = sD;
         pw[p.dim] = sb;
     }
@@ -604,7 +883,7 @@ template <typename T, int LN> __global__ __launch_bounds__(256) void scan_step_k
     y = avsi_group<LN>(y);
     if (ql == 0) {
         if (p.D) y = fmaf(p.D[d], u, y);
-        if (p.z) {
+        if (p.gated) {
             const float z = (float)((const T*)p.z)[b * p.zb + d];
             y *= z * avsi_sigmoid(z);
         }
@@ -612,17 +891,22 @@ template <typename T, int LN> __global__ __launch_bounds__(256) void scan_step_k
     }
 }
 
-int lanes_of(int N) {
-    int l = 1;
-    while (4 * l < N) l *= 2;
-    return l;
+// States with their padding: a power of two from 4 on; MAX_STATE where elements are loaded one by one (fewer than four channels,
+// or states in no whole quads: one form of the kernels for all of those).
+bool by_elements(const avsi_scan_args* a) { return a->dim < 4 || a->state % 4; }
+int padded(const avsi_scan_args* a) {
+    int n = by_elements(a) ? MAX_STATE : 4;
+    while (n < a->state) n *= 2;
+    return n;
 }
+int lanes_of(const avsi_scan_args* a) { return padded(a) / 4; }
+int step_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 int block_channels(int LN) { return LN <= 4 ? 64 : 256 / LN; }
 
 // Chunks of time: none where the batch and the channels leave a wave for each of the 1024 SIMDs -- the first launch over the chunks
 // costs three quarters of the main one --, else as many as make two, of at least 64 steps.
 void chunks_of(const avsi_scan_args* a, int* chunk, int* chunks) {
-    const int LN = lanes_of(a->state), CH = block_channels(LN);
+    const int LN = lanes_of(a), CH = block_channels(LN);
     const int64_t waves = (int64_t)a->batch * a->groups * avsi_ceil_div(a->dim / a->groups, CH) * (CH * LN / 64);
     int64_t n = waves >= 1024 ? 1 : avsi_ceil_div(2048, waves);
     const int64_t most = avsi_ceil_div(a->time, 64);
@@ -636,6 +920,14 @@ bool shape_ok(const avsi_scan_args* a) {
            a->groups > 0 && a->dim % a->groups == 0;
 }
 
+// A tile's rows are addressed with 32 bits from its first one.
+bool strides_ok(const avsi_scan_args* a) {
+    const int64_t most = (int64_t)1 << 26;
+    for (int64_t s : {a->u_stride[1], a->dt_stride[1], a->z_stride[1], a->dout_stride[1], a->out_stride[1], a->B_stride[1], a->C_stride[1]})
+        if (s < 0 || s > most) return false;
+    return true;
+}
+
 Scan params(const avsi_scan_args* a) {
     Scan p = {};
     p.u = a->u, p.dt = a->dt, p.z = a->z, p.B = a->B, p.C = a->C, p.dout = a->dout;
@@ -645,32 +937,36 @@ Scan params(const avsi_scan_args* a) {
     p.Cb = a->C_stride[0], p.Ct = a->C_stride[1], p.Cg = a->C_stride[2];
     p.ob = a->out_stride[0], p.ot = a->out_stride[1];
     p.A = a->A, p.D = a->D, p.bias = a->dt_bias, p.state = a->state_in, p.state_out = a->state_out;
+    p.gated = a->z != nullptr;
+    if (!p.gated) p.z = p.u, p.zb = p.ub, p.zt = p.ut;         // (read in its place, and not used)
     p.lengths = a->lengths, p.out = a->out, p.kept = a->kept, p.du = a->du, p.ddt = a->ddt, p.dz = a->dz;
-    p.batch = a->batch, p.T = a->time, p.dim = a->dim, p.N = a->state, p.groups = a->groups, p.softplus = a->softplus;
+    p.batch = a->batch, p.T = a->time, p.dim = a->dim, p.N = a->state, p.NP = padded(a), p.groups = a->groups, p.softplus = a->softplus;
     chunks_of(a, &p.chunk, &p.chunks);
-    p.blocks = (int)avsi_ceil_div(a->dim / a->groups, block_channels(lanes_of(a->state)));
+    p.blocks = (int)avsi_ceil_div(a->dim / a->groups, block_channels(lanes_of(a)));
     return p;
 }
 
 size_t chunk_floats(const avsi_scan_args* a, int chunks) {
-    return chunks < 2 ? 0 : (size_t)a->batch * chunks * a->dim * (4 * lanes_of(a->state) + 1);
+    return chunks < 2 ? 0 : (size_t)a->batch * chunks * a->dim * (padded(a) + 1);
 }
 
-template <typename T, int LN> void go_fwd(const Scan& p, hipStream_t s) {
-    const dim3 wg(Shape<LN>::NT);
-    if (p.chunks > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, LN, false>), dim3(p.groups * p.blocks, p.chunks - 1, p.batch), wg, 0, s, p);
-        hipLaunchKernelGGL((scan_join_kernel<LN, false>), dim3(avsi_ceil_div((int64_t)p.batch * p.dim * LN, 256)), dim3(256), 0, s, p);
-    }
-    hipLaunchKernelGGL((scan_fwd_kernel<T, LN>), dim3(p.groups * p.blocks, p.chunks, p.batch), wg, 0, s, p);
+template <bool BACK> void go_join(const Scan& p, hipStream_t s) {
+    const int QB = p.NP / 4;
+    hipLaunchKernelGGL(scan_join_kernel<BACK>, dim3(avsi_ceil_div((int64_t)p.batch * p.dim * QB, 256)), dim3(256), 0, s, p, QB);
 }
-template <typename T, int LN> void go_bwd(const Scan& p, hipStream_t s) {
-    const dim3 wg(Shape<LN>::NT);
+template <typename T, typename S> void go_fwd(const Scan& p, hipStream_t s) {
     if (p.chunks > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, LN, true>), dim3(p.groups * p.blocks, p.chunks - 1, p.batch), wg, 0, s, p);
-        hipLaunchKernelGGL((scan_join_kernel<LN, true>), dim3(avsi_ceil_div((int64_t)p.batch * p.dim * LN, 256)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((scan_chunk_kernel<T, S, false>), dim3(p.groups * p.blocks, p.chunks - 1, p.batch), dim3(2 * S::NT), 0, s, p);
+        go_join<false>(p, s);
     }
-    hipLaunchKernelGGL((scan_bwd_kernel<T, LN>), dim3(p.groups * p.blocks, p.chunks, p.batch), wg, 0, s, p);
+    hipLaunchKernelGGL((scan_fwd_kernel<T, S>), dim3(p.groups * p.blocks, p.chunks, p.batch), dim3(2 * S::NT), 0, s, p);
+}
+template <typename T, typename S> void go_bwd(const Scan& p, hipStream_t s) {
+    if (p.chunks > 1) {
+        hipLaunchKernelGGL((scan_chunk_kernel<T, S, true>), dim3(p.groups * p.blocks, p.chunks - 1, p.batch), dim3(2 * S::NT), 0, s, p);
+        go_join<true>(p, s);
+    }
+    hipLaunchKernelGGL((scan_bwd_kernel<T, S>), dim3(p.groups * p.blocks, p.chunks, p.batch), dim3(2 * S::NT), 0, s, p);
 }
 template <typename T, int LN> void go_step(const Scan& p, hipStream_t s) {
     hipLaunchKernelGGL((scan_step_kernel<T, LN>), dim3(avsi_ceil_div((int64_t)p.batch * p.dim * LN, 256)), dim3(256), 0, s, p);
@@ -678,22 +974,31 @@ template <typename T, int LN> void go_step(const Scan& p, hipStream_t s) {
 
 }  // namespace
 
-#define AVSI_SCAN_LN(T, GO)         \
-    switch (lanes_of(a->state)) {   \
-        case 1: GO<T, 1>(p, s); break;   \
-        case 2: GO<T, 2>(p, s); break;   \
-        case 4: GO<T, 4>(p, s); break;   \
-        case 8: GO<T, 8>(p, s); break;   \
+#define AVSI_SCAN_N(T, GO)                               \
+    switch (by_elements(a) ? 0 : padded(a)) {            \
+        case 0: GO<T, Shape<16, 4, true>>(p, s); break;  \
+        case 4: GO<T, Shape<1, 4>>(p, s); break;         \
+        case 8: GO<T, Shape<2, 4>>(p, s); break;         \
+        case 16: GO<T, Shape<4, 4>>(p, s); break;        \
+        case 32: GO<T, Shape<8, 4>>(p, s); break;        \
+        default: GO<T, Shape<16, 4>>(p, s); break;       \
+    }
+#define AVSI_STEP_N(T, GO)               \
+    switch (step_states(a->state)) { \
+        case 4: GO<T, 1>(p, s); break;   \
+        case 8: GO<T, 2>(p, s); break;   \
+        case 16: GO<T, 4>(p, s); break;  \
+        case 32: GO<T, 8>(p, s); break;  \
         default: GO<T, 16>(p, s); break; \
     }
-#define AVSI_SCAN_T(GO)                                         \
-    if (a->dtype == AVSI_F32) { AVSI_SCAN_LN(float, GO) }       \
-    else if (a->dtype == AVSI_BF16) { AVSI_SCAN_LN(__bf16, GO) } \
-    else { AVSI_SCAN_LN(_Float16, GO) }
+#define AVSI_SCAN_T(BY_N, GO)                          \
+    if (a->dtype == AVSI_F32) { BY_N(float, GO) }      \
+    else if (a->dtype == AVSI_BF16) { BY_N(__bf16, GO) } \
+    else { BY_N(_Float16, GO) }
 
 extern "C" size_t avsi_selective_scan_kept_floats(const avsi_scan_args* a) {
     if (!shape_ok(a) || a->state > MAX_STATE) return 0;
-    return (size_t)a->batch * avsi_ceil_div(a->time, TT) * a->dim * 4 * lanes_of(a->state);
+    return (size_t)a->batch * avsi_ceil_div(a->time, TT) * a->dim * padded(a);
 }
 
 extern "C" size_t avsi_selective_scan_workspace_bytes(const avsi_scan_args* a) {
@@ -705,22 +1010,22 @@ extern "C" size_t avsi_selective_scan_workspace_bytes(const avsi_scan_args* a) {
 
 extern "C" int avsi_selective_scan(const avsi_scan_args* a, void* workspace, size_t workspace_bytes, void* stream) {
     if (!shape_ok(a) || !a->u || !a->dt || !a->A || !a->B || !a->C || !a->out) return AVSI_ERR_INVALID_ARG;
-    if (a->state > MAX_STATE) return AVSI_ERR_UNSUPPORTED;
+    if (a->state > MAX_STATE || !strides_ok(a)) return AVSI_ERR_UNSUPPORTED;
     const size_t need = avsi_selective_scan_workspace_bytes(a);
     if (need && (!workspace || workspace_bytes < need)) return AVSI_ERR_WORKSPACE;
     Scan p = params(a);
     p.ends = (float*)workspace;
-    p.sums = p.ends ? p.ends + (size_t)p.batch * p.chunks * p.dim * 4 * lanes_of(p.N) : nullptr;
+    p.sums = p.ends ? p.ends + (size_t)p.batch * p.chunks * p.dim * p.NP : nullptr;
     hipStream_t s = (hipStream_t)stream;
     avsi_clear_error();
-    AVSI_SCAN_T(go_fwd)
+    AVSI_SCAN_T(AVSI_SCAN_N, go_fwd)
     return avsi_launch_status();
 }
 
 extern "C" size_t avsi_selective_scan_bwd_workspace_bytes(const avsi_scan_args* a) {
     if (!shape_ok(a) || a->state > MAX_STATE) return 0;
     const Scan p = params(a);
-    const size_t NP = 4 * lanes_of(p.N);
+    const size_t NP = p.NP;
     return (chunk_floats(a, p.chunks) + (size_t)p.batch * p.T * p.groups * p.blocks * 2 * NP +
             (size_t)p.batch * p.chunks * partial_stride(p.dim, NP)) * sizeof(float);
 }
@@ -729,10 +1034,10 @@ extern "C" int avsi_selective_scan_bwd(const avsi_scan_args* a, void* workspace,
     if (!shape_ok(a) || !a->u || !a->dt || !a->A || !a->B || !a->C || !a->dout || !a->kept || !a->du || !a->ddt || !a->dA || !a->dB ||
         !a->dC || !a->z != !a->dz)
         return AVSI_ERR_INVALID_ARG;
-    if (a->state > MAX_STATE) return AVSI_ERR_UNSUPPORTED;
+    if (a->state > MAX_STATE || !strides_ok(a)) return AVSI_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < avsi_selective_scan_bwd_workspace_bytes(a)) return AVSI_ERR_WORKSPACE;
     Scan p = params(a);
-    const int NP = 4 * lanes_of(p.N);
+    const int NP = p.NP;
     // (every part is a multiple of four floats but the sums of the chunks: they come last)
     p.part_bc = (float*)workspace;
     p.part_w = p.part_bc + (size_t)p.batch * p.T * p.groups * p.blocks * 2 * NP;
@@ -740,7 +1045,7 @@ extern "C" int avsi_selective_scan_bwd(const avsi_scan_args* a, void* workspace,
     p.sums = p.ends + (size_t)p.batch * p.chunks * p.dim * NP;
     hipStream_t s = (hipStream_t)stream;
     avsi_clear_error();
-    AVSI_SCAN_T(go_bwd)
+    AVSI_SCAN_T(AVSI_SCAN_N, go_bwd)
     const int64_t bc = (int64_t)p.batch * p.T * p.groups * 2 * NP;
     const dim3 grid(avsi_ceil_div(bc, 256));
     if (a->dtype == AVSI_F32)
@@ -756,10 +1061,10 @@ extern "C" int avsi_selective_scan_bwd(const avsi_scan_args* a, void* workspace,
 
 extern "C" int avsi_selective_scan_step(const avsi_scan_args* a, void* stream) {
     if (!shape_ok(a) || a->time != 1 || !a->u || !a->dt || !a->A || !a->B || !a->C || !a->out || !a->state_out) return AVSI_ERR_INVALID_ARG;
-    if (a->state > MAX_STATE) return AVSI_ERR_UNSUPPORTED;
+    if (a->state > MAX_STATE || !strides_ok(a)) return AVSI_ERR_UNSUPPORTED;
     Scan p = params(a);
     hipStream_t s = (hipStream_t)stream;
     avsi_clear_error();
-    AVSI_SCAN_T(go_step)
+    AVSI_SCAN_T(AVSI_STEP_N, go_step)
     return avsi_launch_status();
 }
