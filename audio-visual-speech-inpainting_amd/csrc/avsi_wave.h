@@ -96,6 +96,33 @@ template <typename T> struct avsi_quad {
     }
 };
 
+// V elements as words: the same for pieces of V * sizeof(T) bytes.
+template <typename T, int V> struct avsi_pack {
+    static constexpr int WORDS = V * sizeof(T) / 4;
+    typedef __attribute__((ext_vector_type(WORDS))) unsigned W;
+    W v;
+    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(&v, p, sizeof(v)); }
+    __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, &v, sizeof(v)); }
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, (unsigned)v[i]);
+        const unsigned w = v[i / 2];
+        if constexpr (__is_same(T, __bf16)) return __builtin_bit_cast(float, i & 1 ? w & 0xffff0000u : w << 16);
+        typedef __attribute__((ext_vector_type(2))) _Float16 half2;
+        return (float)__builtin_bit_cast(half2, w)[i & 1];
+    }
+    __device__ __forceinline__ void set(const float (&f)[V]) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __builtin_bit_cast(unsigned, f[i]);
+            } else {
+                typedef __attribute__((ext_vector_type(2))) T Pair;
+                v[i] = __builtin_bit_cast(unsigned, Pair{(T)f[2 * i], (T)f[2 * i + 1]});
+            }
+        }
+    }
+};
+
 // A lane permutation inside rows of 16 as a VALU operand (no LDS).
 template <int CTRL> __device__ __forceinline__ float avsi_dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -124,6 +151,34 @@ template <int G, typename OP = avsi_add> __device__ __forceinline__ float avsi_g
     if (G >= 32) { float a = v, b = v; avsi_swap16(a, b); v = OP::of(a, b); }
     if (G >= 64) { float a = v, b = v; avsi_swap32(a, b); v = OP::of(a, b); }
     return v;
+}
+
+// Column c = 32 blockIdx.x + (threadIdx.x & 31) of P rows of partials, added by a workgroup of 1024: 32 slices of the rows, eight loads
+// of a slice in flight, then the slices, all in a fixed order.  The sum is in the first 32 threads.
+__device__ __forceinline__ float avsi_column_sum(const float* __restrict__ part, int P, int64_t stride, int64_t cols) {
+    __shared__ float lds[32][33];
+    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int slice = threadIdx.x >> 5;
+    float s = 0.f;
+    if (c < cols) {
+        const float* at = part + c;
+        int r = slice;
+        for (; r + 7 * 32 < P; r += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = at[(int64_t)(r + 32 * i) * stride];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
+        for (; r < P; r += 32) s += at[(int64_t)r * stride];
+    }
+    lds[slice][threadIdx.x & 31] = s;
+    __syncthreads();
+    s = 0.f;
+    if (threadIdx.x < 32)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += lds[i][threadIdx.x];
+    return s;
 }
 
 // Functions of the gates, to a few ulp, on the hardware's base-2 exponential.  In softplus x log2 e is carried in two words; then

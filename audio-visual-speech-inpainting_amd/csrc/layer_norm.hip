@@ -4,10 +4,13 @@
 //   backward: e = dy gamma,  dx = rstd (e - mean(e) - h mean(e h)),  dgamma = sum over rows of dy h,  dbeta = sum over rows of dy
 //
 // Both passes are bound by memory: x in and y out (forward), x and dy in and dx out (backward).  A row is read ONCE into the
-// registers of its group of lanes -- 16, 64, 256 or 1024 lanes, the fewest that hold it in at most four 16-byte pieces each -- and
-// the variance is the second pass over those registers (a one-pass sum of squares would cancel where the mean is large).  Rows
-// beyond 1024 x 4 pieces are streamed: each pass over the row reads it again, from L2.  A group walks the rows r, r + groups, ...
-// and keeps its slice of gamma (and beta) in registers.
+// registers of its group of lanes -- 16, 64, 256 or 1024 lanes with one to four 16-byte pieces each --
+// and the variance is the second pass over those registers (a one-pass sum of squares would cancel where the mean is large).  The
+// next row's loads are issued before this row's sums.  Rows beyond 1024 x 2 pieces are streamed: each pass over the row reads it
+// again, from L2.  A group walks the rows r, r + groups, ... and keeps its slice of gamma (and beta) in registers.
+//
+// Widths in no whole pieces: the lane that the row's end cuts takes the last whole piece of the row instead, which overlaps its
+// neighbour's; what both hold is counted once and written twice, with the same value.  (A branch around the load would wait for it.)
 //
 // Weight gradients: every lane owns the same columns in all its rows, so dgamma and dbeta are sums in its registers; the groups of a
 // workgroup are added in LDS in a fixed order, workgroups through partials [P][2][C] in the workspace and a second launch: no
@@ -17,72 +20,124 @@
 
 namespace {
 
-constexpr int NV = 4;       // 16-byte pieces of a row per lane
-
-// Sum over the L lanes of a group (L <= 64: inside a wave; else the whole workgroup, through LDS).
-template <int L> __device__ __forceinline__ float group_sum(float v, float* lds) {
-    if (L <= 64) return avsi_group<L < 64 ? L : 64>(v);
-    v = avsi_group<64>(v);
-    __syncthreads();                        // the sums of the previous call have been read
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = 0.f;
+// Sums over the L lanes of a group: inside a wave, or over the whole workgroup through LDS.  Two buffers in turn: a wave that writes
+// one again has passed the barrier behind which the other was read.  (The barrier waits for LDS only: loads stay in flight.)
+template <int L> struct Sums {
+    avsi_f2 lds[L > 64 ? 2 : 1][L > 64 ? L / 64 : 1];
+};
+template <int L> __device__ __forceinline__ avsi_f2 group_sums(float v, float w, Sums<L>& sums, int& turn) {
+    v = avsi_group<L < 64 ? L : 64>(v);
+    w = avsi_group<L < 64 ? L : 64>(w);
+    if (L <= 64) return avsi_f2{v, w};
+    if ((threadIdx.x & 63) == 0) sums.lds[turn][threadIdx.x >> 6] = avsi_f2{v, w};
+    AVSI_LDS_BARRIER();
+    avsi_f2 s = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < L / 64; ++i) s += lds[i];
+    for (int i = 0; i < L / 64; ++i) {
+        s[0] += sums.lds[turn][i][0];
+        s[1] += sums.lds[turn][i][1];
+    }
+    turn ^= 1;
     return s;
 }
 
-template <typename T, typename W, int L>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void ln_fwd_kernel(const T* __restrict__ x, int64_t xs, const W* __restrict__ gamma,
-                                                                    const W* __restrict__ beta, T* __restrict__ y, int64_t ys,
-                                                                    float* __restrict__ mean, float* __restrict__ rstd, int64_t rows,
-                                                                    int C, float eps) {
-    constexpr int V = 16 / sizeof(T);
-    constexpr int PER_WG = (L < 256 ? 256 : L) / L;
-    __shared__ float lds[L > 64 ? L / 64 : 1];
-    const int lane = threadIdx.x % L;
-    const float fc = (float)C;
-    avsi_raw<W, V> gr[NV], br[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = (j * L + lane) * V;
-        if (gamma) gr[j] = avsi_load_raw<W, V>(gamma + c, C - c);
-        if (beta) br[j] = avsi_load_raw<W, V>(beta + c, C - c);
-    }
-    for (int64_t r = (int64_t)blockIdx.x * PER_WG + threadIdx.x / L; r < rows; r += (int64_t)gridDim.x * PER_WG) {
-        float v[NV][V];
-        float s = 0.f;
+// Where a lane's pieces lie: piece j starts at column c[j] and its elements from skip[j] on are its own.
+template <typename T, int L, int NV, bool SMALL> struct Pieces {
+    static constexpr int V = 16 / sizeof(T);
+    int c[NV], skip[NV];
+    __device__ __forceinline__ Pieces(int lane, int C) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * L + lane) * V;
-            avsi_load<T, V>(x + r * xs + c, C - c, v[j]);
+            const int at = (j * L + lane) * V;
+            c[j] = SMALL ? at : (at < C - V ? at : C - V);
+            skip[j] = SMALL ? 0 : at - c[j];
         }
+    }
+    __device__ __forceinline__ bool own(int j, int i, int C) const { return SMALL ? c[j] + i < C : i >= skip[j]; }
+    __device__ __forceinline__ bool any(int j, int C) const { return SMALL ? c[j] < C : skip[j] < V; }
+    // a piece of a row, or of a weight, in the elements' type
+    template <typename E> __device__ __forceinline__ void load(const E* row, int j, int C, avsi_pack<E, V>& v) const {
+        if (!SMALL) {
+            v.load(row + c[j]);
+        } else {                        // (fewer columns than a piece has)
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = (float)row[c[j] + i < C ? c[j] + i : C - 1];
+            v.set(f);
+        }
+    }
+    template <typename E> __device__ __forceinline__ void store(E* row, int j, int C, const float (&f)[V]) const {
+        if (!any(j, C)) return;
+        if (!SMALL) {
+            avsi_pack<E, V> v;
+            v.set(f);
+            v.store(row + c[j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (c[j] + i < C) row[c[j] + i] = (E)f[i];
+        }
+    }
+};
+
+template <int L> constexpr int threads() { return L < 256 ? 256 : L; }
+
+template <typename T, typename W, int L, int NV, bool SMALL>
+__global__ __launch_bounds__(threads<L>()) void ln_fwd_kernel(const T* __restrict__ x, int64_t xs, const W* __restrict__ gamma,
+                                                               const W* __restrict__ beta, T* __restrict__ y, int64_t ys,
+                                                               float* __restrict__ mean, float* __restrict__ rstd, int64_t rows, int C,
+                                                               float eps) {
+    constexpr int V = 16 / sizeof(T), PER_WG = threads<L>() / L;
+    __shared__ Sums<L> sums;
+    int turn = 0;
+    const int lane = threadIdx.x % L;
+    const Pieces<T, L, NV, SMALL> at(lane, C);
+    const float fc = (float)C;
+    avsi_pack<W, V> gr[NV], br[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        if (gamma) at.load(gamma, j, C, gr[j]);
+        if (beta) at.load(beta, j, C, br[j]);
+    }
+    const int64_t step = (int64_t)gridDim.x * PER_WG;
+    int64_t r = (int64_t)blockIdx.x * PER_WG + threadIdx.x / L;
+    avsi_pack<T, V> next[NV];
+    if (r < rows)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) at.load(x + r * xs, j, C, next[j]);
+    for (; r < rows; r += step) {
+        float v[NV][V], s = 0.f, q = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) s += v[j][i];           // (columns behind the row's end are zero)
-        const float mu = group_sum<L>(s, lds) / fc;
-        float q = 0.f;
+            for (int i = 0; i < V; ++i) v[j][i] = next[j].at(i);
+        const int64_t ahead = r + step < rows ? r + step : r;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) at.load(x + ahead * xs, j, C, next[j]);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) s += at.own(j, i, C) ? v[j][i] : 0.f;
+        const float mu = group_sums<L>(s, 0.f, sums, turn)[0] / fc;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float d = (j * L + lane) * V + i < C ? v[j][i] - mu : 0.f;
+                v[j][i] -= mu;
+                const float d = at.own(j, i, C) ? v[j][i] : 0.f;
                 q = fmaf(d, d, q);
             }
-        const float rs = 1.f / sqrtf(group_sum<L>(q, lds) / fc + eps);
+        const float rs = 1.f / sqrtf(group_sums<L>(q, 0.f, sums, turn)[0] / fc + eps);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * L + lane) * V;
-            if (c >= C) continue;
             float o[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                o[i] = (v[j][i] - mu) * rs;
-                if (gamma) o[i] *= (float)gr[j].v[i];
-                if (beta) o[i] += (float)br[j].v[i];
+                o[i] = v[j][i] * rs;
+                if (gamma) o[i] *= gr[j].at(i);
+                if (beta) o[i] += br[j].at(i);
             }
-            avsi_store<T, V>(y + r * ys + c, C - c, o);
+            at.store(y + r * ys, j, C, o);
         }
         if (lane == 0) {
             mean[r] = mu;
@@ -98,7 +153,8 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* __restrict__
                                                            float* __restrict__ mean, float* __restrict__ rstd, int64_t rows, int C,
                                                            float eps) {
     constexpr int V = 16 / sizeof(T), L = 1024;
-    __shared__ float lds[L / 64];
+    __shared__ Sums<L> sums;
+    int turn = 0;
     const float fc = (float)C;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const T* xr = x + r * xs;
@@ -108,7 +164,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* __restrict__
 #pragma unroll
             for (int i = 0; i < V; ++i) s += v[i];
         }
-        const float mu = group_sum<L>(s, lds) / fc;
+        const float mu = group_sums<L>(s, 0.f, sums, turn)[0] / fc;
         for (int c = threadIdx.x * V; c < C; c += L * V) {
             avsi_load<T, V>(xr + c, C - c, v);
 #pragma unroll
@@ -117,7 +173,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* __restrict__
                 q = fmaf(d, d, q);
             }
         }
-        const float rs = 1.f / sqrtf(group_sum<L>(q, lds) / fc + eps);
+        const float rs = 1.f / sqrtf(group_sums<L>(q, 0.f, sums, turn)[0] / fc + eps);
         for (int c = threadIdx.x * V; c < C; c += L * V) {
             float g[V], b[V];
             avsi_load<T, V>(xr + c, C - c, v);
@@ -138,58 +194,71 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* __restrict__
     }
 }
 
-template <typename T, typename W, int L, bool WGRAD>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void ln_bwd_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x,
-                                                                    int64_t xs, const float* __restrict__ mean,
-                                                                    const float* __restrict__ rstd, const W* __restrict__ gamma,
-                                                                    T* __restrict__ dx, int64_t dxs, float* __restrict__ part,
-                                                                    int64_t rows, int C) {
-    constexpr int V = 16 / sizeof(T);
-    constexpr int NT = L < 256 ? 256 : L, PER_WG = NT / L;
-    __shared__ float lds[L > 64 ? L / 64 : 1];
+template <typename T, typename W, int L, int NV, bool SMALL, bool WGRAD>
+__global__ __launch_bounds__(threads<L>()) void ln_bwd_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs,
+                                                               const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                               const W* __restrict__ gamma, T* __restrict__ dx, int64_t dxs,
+                                                               float* __restrict__ part, int64_t rows, int C) {
+    constexpr int V = 16 / sizeof(T), PER_WG = threads<L>() / L;
+    __shared__ Sums<L> sums;
+    int turn = 0;
     __shared__ float acc[WGRAD && PER_WG > 1 ? 2 * L * V * NV : 1];
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
+    const Pieces<T, L, NV, SMALL> at(lane, C);
     const float inv = 1.f / (float)C;
-    avsi_raw<W, V> gr[NV];
+    avsi_pack<W, V> gr[NV];
     float dg[NV][V], db[NV][V];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (j * L + lane) * V;
-        if (gamma) gr[j] = avsi_load_raw<W, V>(gamma + c, C - c);
+        if (gamma) at.load(gamma, j, C, gr[j]);
 #pragma unroll
         for (int i = 0; i < V; ++i) dg[j][i] = db[j][i] = 0.f;
     }
-    for (int64_t r = (int64_t)blockIdx.x * PER_WG + group; r < rows; r += (int64_t)gridDim.x * PER_WG) {
-        float h[NV][V], g[NV][V];
+    const int64_t step = (int64_t)gridDim.x * PER_WG;
+    int64_t r = (int64_t)blockIdx.x * PER_WG + group;
+    avsi_pack<T, V> nx[NV], ng[NV];
+    float nmu = 0.f, nrs = 0.f;
+    auto load = [&](int64_t row) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * L + lane) * V;
-            avsi_load<T, V>(x + r * xs + c, C - c, h[j]);
-            avsi_load<T, V>(dy + r * dys + c, C - c, g[j]);
+            at.load(x + row * xs, j, C, nx[j]);
+            at.load(dy + row * dys, j, C, ng[j]);
         }
-        const float mu = mean[r], rs = rstd[r];
-        float s1 = 0.f, s2 = 0.f;
+        nmu = mean[row];
+        nrs = rstd[row];
+    };
+    if (r < rows) load(r);
+    for (; r < rows; r += step) {
+        float h[NV][V], g[NV][V], s1 = 0.f, s2 = 0.f;
+        const float mu = nmu, rs = nrs;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                h[j][i] = (h[j][i] - mu) * rs;          // (behind the row's end dy is zero, and with it every term)
+                h[j][i] = (nx[j].at(i) - mu) * rs;
+                g[j][i] = ng[j].at(i);
+            }
+        load(r + step < rows ? r + step : r);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
                 if (WGRAD) {
                     dg[j][i] = fmaf(g[j][i], h[j][i], dg[j][i]);
                     db[j][i] += g[j][i];
                 }
-                if (gamma) g[j][i] *= (float)gr[j].v[i];
-                s1 += g[j][i];
-                s2 = fmaf(g[j][i], h[j][i], s2);
+                if (gamma) g[j][i] *= gr[j].at(i);
+                const float e = at.own(j, i, C) ? g[j][i] : 0.f;
+                s1 += e;
+                s2 += at.own(j, i, C) ? e * h[j][i] : 0.f;
             }
-        const float m1 = group_sum<L>(s1, lds) * inv, m2 = group_sum<L>(s2, lds) * inv;
+        const avsi_f2 both = group_sums<L>(s1, s2, sums, turn);
+        const float m1 = both[0] * inv, m2 = both[1] * inv;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * L + lane) * V;
-            if (c >= C) continue;
 #pragma unroll
             for (int i = 0; i < V; ++i) g[j][i] = (g[j][i] - m1 - h[j][i] * m2) * rs;
-            avsi_store<T, V>(dx + r * dxs + c, C - c, g[j]);
+            at.store(dx + r * dxs, j, C, g[j]);
         }
     }
     if (!WGRAD) return;
@@ -199,10 +268,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_bwd_kernel(const T* __re
         if (group != k) continue;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * L + lane) * V;
-            if (c >= C) continue;
             if (PER_WG > 1) {
-                float* a = acc + 2 * c;
+                float* a = acc + 2 * V * (j * L + lane);
                 if (k > 0)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
@@ -217,9 +284,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_bwd_kernel(const T* __re
                     }
             }
             if (k == PER_WG - 1) {
-                float* p = part + (int64_t)blockIdx.x * 2 * C + c;
-                avsi_store<float, V>(p, C - c, dg[j]);
-                avsi_store<float, V>(p + C, C - c, db[j]);
+                at.store(part + (int64_t)blockIdx.x * 2 * C, j, C, dg[j]);
+                at.store(part + (int64_t)blockIdx.x * 2 * C + C, j, C, db[j]);
             }
         }
     }
@@ -232,13 +298,18 @@ __global__ __launch_bounds__(1024) void ln_bwd_wide_kernel(const T* __restrict__
                                                            const W* __restrict__ gamma, T* __restrict__ dx, int64_t dxs, int64_t rows,
                                                            int C) {
     constexpr int V = 16 / sizeof(T), L = 1024;
-    __shared__ float lds[L / 64];
+    __shared__ Sums<L> sums;
+    int turn = 0;
     const float inv = 1.f / (float)C;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const float mu = mean[r], rs = rstd[r];
         float s1 = 0.f, s2 = 0.f, h[V], g[V], w[V];
         for (int pass = 0; pass < 2; ++pass) {
-            const float m1 = pass ? group_sum<L>(s1, lds) * inv : 0.f, m2 = pass ? group_sum<L>(s2, lds) * inv : 0.f;
+            float m1 = 0.f, m2 = 0.f;
+            if (pass) {
+                const avsi_f2 both = group_sums<L>(s1, s2, sums, turn);
+                m1 = both[0] * inv, m2 = both[1] * inv;
+            }
             for (int c = threadIdx.x * V; c < C; c += L * V) {
                 avsi_load<T, V>(x + r * xs + c, C - c, h);
                 avsi_load<T, V>(dy + r * dys + c, C - c, g);
@@ -285,29 +356,29 @@ __global__ __launch_bounds__(256) void ln_wgrad_wide_kernel(const T* __restrict_
     avsi_store<float, V>(p + C, C - c, db);
 }
 
-// out[c] = sum over p of part[p][c], c < 2 C: 16 columns x 16 slices of the partials per workgroup.
-__global__ __launch_bounds__(256) void ln_wgrad_sum_kernel(const float* __restrict__ part, int P, int C, float* __restrict__ dgamma,
-                                                           float* __restrict__ dbeta) {
-    __shared__ float lds[256];
-    const int c = blockIdx.x * 16 + (threadIdx.x & 15);
-    float s = 0.f;
-    if (c < 2 * C)
-        for (int p = threadIdx.x >> 4; p < P; p += 16) s += part[(int64_t)p * 2 * C + c];
-    lds[threadIdx.x] = s;
-    __syncthreads();
-    if (threadIdx.x < 16 && c < 2 * C) {
-        s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s += lds[i * 16 + threadIdx.x];
+// dgamma, dbeta = sums of part[P][2][C].
+__global__ __launch_bounds__(1024) void ln_wgrad_sum_kernel(const float* __restrict__ part, int P, int C, float* __restrict__ dgamma,
+                                                            float* __restrict__ dbeta) {
+    const float s = avsi_column_sum(part, P, 2 * (int64_t)C, 2 * (int64_t)C);
+    const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x < 32 && c < 2 * (int64_t)C) {
         if (c < C) dgamma[c] = s;
         else dbeta[c - C] = s;
     }
 }
 
-// Lanes of a row's group: the fewest of 16, 64, 256, 1024 that hold C columns; 0: none does.
-int group_lanes(int C, int dtype) {
-    const int piece = 16 / avsi_dtype_size(dtype) * NV;
-    return C <= 16 * piece ? 16 : C <= 64 * piece ? 64 : C <= 256 * piece ? 256 : C <= 1024 * piece ? 1024 : 0;
+// The group of lanes that a row of C columns takes, and its pieces per lane; 0 lanes: none holds it.  Four pieces only in the
+// forward pass: the backward pass holds two rows and two sums per column.
+struct Group { int L, NV; };
+Group group_of(int C, int dtype, bool back) {
+    const int V = 16 / avsi_dtype_size(dtype);
+    const int64_t n = avsi_ceil_div(C, V);
+    if (n <= 16) return {16, 1};
+    if (n <= 128) return {64, n <= 64 ? 1 : 2};
+    if (n <= 256) return back ? Group{256, 1} : Group{64, 4};
+    if (n <= 512) return {256, 2};
+    if (n <= 1024) return back ? Group{1024, 1} : Group{256, 4};
+    return n <= 2048 ? Group{1024, 2} : Group{0, 0};
 }
 
 int fwd_groups(int64_t rows, int L) {
@@ -318,27 +389,36 @@ int fwd_groups(int64_t rows, int L) {
 
 // Workgroups of the backward pass = partials of the weights' gradients.
 int bwd_groups(int64_t rows, int C, int dtype) {
-    const int L = group_lanes(C, dtype);
+    const int L = group_of(C, dtype, true).L;
     if (!L) return (int)(rows < 64 ? rows : 64);
     const int per_wg = L < 256 ? 256 / L : 1;
     const int64_t wgs = avsi_ceil_div(rows, per_wg), most = 2 * AVSI_NUM_CU;
     return (int)(wgs < most ? wgs : most);
 }
 
+#define AVSI_LN_SHAPES(GO, BIG)                         \
+    if (C < 16 / (int)sizeof(T)) GO(16, 1, true);       \
+    else if (g.L == 16) GO(16, 1, false);               \
+    else if (g.L == 64 && g.NV == 1) GO(64, 1, false);  \
+    else if (g.L == 64 && g.NV == 2) GO(64, 2, false);  \
+    else if (g.L == 256 && g.NV == 2) GO(256, 2, false); \
+    else if (g.L == 1024 && g.NV == 2) GO(1024, 2, false); \
+    else BIG(GO)
+#define AVSI_LN_BIG_FWD(GO) if (g.L == 64) GO(64, 4, false); else GO(256, 4, false)
+#define AVSI_LN_BIG_BWD(GO) if (g.L == 256) GO(256, 1, false); else GO(1024, 1, false)
+
 template <typename T, typename W>
 int launch_fwd(const void* x, int64_t xs, const void* gamma, const void* beta, void* y, int64_t ys, float* mean, float* rstd,
-               int64_t rows, int C, float eps, int L, hipStream_t s) {
-    const dim3 grid(fwd_groups(rows, L));
-#define AVSI_LN_FWD(LANES, NT)                                                                                                       \
-    hipLaunchKernelGGL((ln_fwd_kernel<T, W, LANES>), grid, dim3(NT), 0, s, (const T*)x, xs, (const W*)gamma, (const W*)beta, (T*)y, \
-                       ys, mean, rstd, rows, C, eps)
-    if (L == 16) AVSI_LN_FWD(16, 256);
-    else if (L == 64) AVSI_LN_FWD(64, 256);
-    else if (L == 256) AVSI_LN_FWD(256, 256);
-    else if (L == 1024) AVSI_LN_FWD(1024, 1024);
-    else
+               int64_t rows, int C, float eps, int dtype, hipStream_t s) {
+    const Group g = group_of(C, dtype, false);
+    const dim3 grid(fwd_groups(rows, g.L));
+#define AVSI_LN_FWD(LANES, PIECES, SMALL)                                                                                            \
+    hipLaunchKernelGGL((ln_fwd_kernel<T, W, LANES, PIECES, SMALL>), grid, dim3(threads<LANES>()), 0, s, (const T*)x, xs,             \
+                       (const W*)gamma, (const W*)beta, (T*)y, ys, mean, rstd, rows, C, eps)
+    if (!g.L)
         hipLaunchKernelGGL((ln_fwd_wide_kernel<T, W>), grid, dim3(1024), 0, s, (const T*)x, xs, (const W*)gamma, (const W*)beta, (T*)y,
                            ys, mean, rstd, rows, C, eps);
+    else { AVSI_LN_SHAPES(AVSI_LN_FWD, AVSI_LN_BIG_FWD); }
 #undef AVSI_LN_FWD
     return avsi_launch_status();
 }
@@ -346,30 +426,29 @@ int launch_fwd(const void* x, int64_t xs, const void* gamma, const void* beta, v
 template <typename T, typename W>
 int launch_bwd(const void* dy, int64_t dys, const void* x, int64_t xs, const float* mean, const float* rstd, const void* gamma,
                void* dx, int64_t dxs, float* dgamma, float* dbeta, float* part, int64_t rows, int C, int dtype, hipStream_t s) {
-    const int L = group_lanes(C, dtype), P = bwd_groups(rows, C, dtype);
-#define AVSI_LN_BWD(LANES, NT, WG)                                                                                                  \
-    hipLaunchKernelGGL((ln_bwd_kernel<T, W, LANES, WG>), dim3(P), dim3(NT), 0, s, (const T*)dy, dys, (const T*)x, xs, mean, rstd,  \
-                       (const W*)gamma, (T*)dx, dxs, part, rows, C)
-#define AVSI_LN_BWD_L(WG)                           \
-    if (L == 16) AVSI_LN_BWD(16, 256, WG);          \
-    else if (L == 64) AVSI_LN_BWD(64, 256, WG);     \
-    else if (L == 256) AVSI_LN_BWD(256, 256, WG);   \
-    else AVSI_LN_BWD(1024, 1024, WG)
-    if (!L) {
+    const Group g = group_of(C, dtype, true);
+    const int P = bwd_groups(rows, C, dtype);
+#define AVSI_LN_BWD(LANES, PIECES, SMALL, WG)                                                                                        \
+    hipLaunchKernelGGL((ln_bwd_kernel<T, W, LANES, PIECES, SMALL, WG>), dim3(P), dim3(threads<LANES>()), 0, s, (const T*)dy, dys,    \
+                       (const T*)x, xs, mean, rstd, (const W*)gamma, (T*)dx, dxs, part, rows, C)
+#define AVSI_LN_BWD_W(LANES, PIECES, SMALL) AVSI_LN_BWD(LANES, PIECES, SMALL, true)
+#define AVSI_LN_BWD_X(LANES, PIECES, SMALL) AVSI_LN_BWD(LANES, PIECES, SMALL, false)
+    if (!g.L) {
         hipLaunchKernelGGL((ln_bwd_wide_kernel<T, W>), dim3(fwd_groups(rows, 0)), dim3(1024), 0, s, (const T*)dy, dys, (const T*)x, xs,
                            mean, rstd, (const W*)gamma, (T*)dx, dxs, rows, C);
         if (dgamma)
             hipLaunchKernelGGL((ln_wgrad_wide_kernel<T>), dim3(avsi_ceil_div(C, 256 * (16 / sizeof(T))), P), dim3(256), 0, s,
                                (const T*)dy, dys, (const T*)x, xs, mean, rstd, part, rows, C);
     } else if (dgamma) {
-        AVSI_LN_BWD_L(true);
+        AVSI_LN_SHAPES(AVSI_LN_BWD_W, AVSI_LN_BIG_BWD);
     } else {
-        AVSI_LN_BWD_L(false);
+        AVSI_LN_SHAPES(AVSI_LN_BWD_X, AVSI_LN_BIG_BWD);
     }
-#undef AVSI_LN_BWD_L
+#undef AVSI_LN_BWD_X
+#undef AVSI_LN_BWD_W
 #undef AVSI_LN_BWD
     if (dgamma)
-        hipLaunchKernelGGL(ln_wgrad_sum_kernel, dim3(avsi_ceil_div(2 * C, 16)), dim3(256), 0, s, part, P, C, dgamma, dbeta);
+        hipLaunchKernelGGL(ln_wgrad_sum_kernel, dim3(avsi_ceil_div(2 * (int64_t)C, 32)), dim3(1024), 0, s, part, P, C, dgamma, dbeta);
     return avsi_launch_status();
 }
 
@@ -384,9 +463,8 @@ extern "C" int avsi_layer_norm(const void* x, int64_t x_stride, int dtype, const
     if (!args_ok(x, x_stride, dtype, wdtype, rows, cols) || !y || y_stride < cols || !mean || !rstd || !(eps >= 0.f))
         return AVSI_ERR_INVALID_ARG;
     avsi_clear_error();
-    const int L = group_lanes(cols, dtype);
     hipStream_t s = (hipStream_t)stream;
-#define AVSI_GO(T, W) return launch_fwd<T, W>(x, x_stride, gamma, beta, y, y_stride, mean, rstd, rows, cols, eps, L, s)
+#define AVSI_GO(T, W) return launch_fwd<T, W>(x, x_stride, gamma, beta, y, y_stride, mean, rstd, rows, cols, eps, dtype, s)
     if (dtype == AVSI_F32) AVSI_GO(float, float);
     if (dtype == AVSI_BF16) {
         if (wdtype == AVSI_F32) AVSI_GO(__bf16, float);

@@ -819,20 +819,12 @@ template <typename T, typename S> __global__ __launch_bounds__(2 * S::NT) void s
     }
 }
 
-// dA [dim][N], dD, ddt_bias [dim] = sums over P partials of [dim][NP], [dim], [dim]: 16 columns x 16 slices per workgroup.
-__global__ __launch_bounds__(256) void scan_wgrad_sum_kernel(const float* __restrict__ part, int P, int dim, int NP, int N,
-                                                             float* __restrict__ dA, float* __restrict__ dD, float* __restrict__ dbias) {
-    __shared__ float lds[256];
-    const int64_t cols = (int64_t)dim * (NP + 2), c = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
-    float s = 0.f;
-    if (c < cols)
-        for (int k = threadIdx.x >> 4; k < P; k += 16) s += part[k * partial_stride(dim, NP) + c];
-    lds[threadIdx.x] = s;
-    __syncthreads();
-    if (threadIdx.x < 16 && c < cols) {
-        s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s += lds[i * 16 + threadIdx.x];
+// dA [dim][N], dD, ddt_bias [dim] = sums over P partials of [dim][NP], [dim], [dim].
+__global__ __launch_bounds__(1024) void scan_wgrad_sum_kernel(const float* __restrict__ part, int P, int dim, int NP, int N,
+                                                              float* __restrict__ dA, float* __restrict__ dD, float* __restrict__ dbias) {
+    const int64_t cols = (int64_t)dim * (NP + 2), c = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    const float s = avsi_column_sum(part, P, partial_stride(dim, NP), cols);
+    if (threadIdx.x < 32 && c < cols) {
         if (c < (int64_t)dim * NP) {
             if (c % NP < N) dA[c / NP * N + c % NP] = s;
         } else if (c < (int64_t)dim * (NP + 1)) {
@@ -1054,7 +1046,7 @@ extern "C" int avsi_selective_scan_bwd(const avsi_scan_args* a, void* workspace,
         hipLaunchKernelGGL((scan_bc_sum_kernel<__bf16>), grid, dim3(256), 0, s, p, NP, (__bf16*)a->dB, (__bf16*)a->dC);
     else
         hipLaunchKernelGGL((scan_bc_sum_kernel<_Float16>), grid, dim3(256), 0, s, p, NP, (_Float16*)a->dB, (_Float16*)a->dC);
-    hipLaunchKernelGGL(scan_wgrad_sum_kernel, dim3(avsi_ceil_div((int64_t)p.dim * (NP + 2), 16)), dim3(256), 0, s, p.part_w,
+    hipLaunchKernelGGL(scan_wgrad_sum_kernel, dim3(avsi_ceil_div((int64_t)p.dim * (NP + 2), 32)), dim3(1024), 0, s, p.part_w,
                        p.batch * p.chunks, p.dim, NP, p.N, a->dA, a->dD, a->ddt_bias);
     return avsi_launch_status();
 }
