@@ -60,13 +60,13 @@ class GemmEpilogue(Structure):
 
 
 class ScanArgs(Structure):
-    """Mirror of ``avsi_scan_args`` (include/avsi_hip.h)."""
+    """Mirror of ``avsi_scan_args`` (include/avsi_hip.h), its arrays of strides field by field."""
     _fields_ = (
         [(n, c_int32) for n in ("dtype", "batch", "time", "dim", "state", "groups", "softplus", "reserved")]
         + [(n, c_void_p) for n in ("u", "dt", "z", "B", "C")]
-        + [(n, c_int64 * k) for n, k in (("u_stride", 2), ("dt_stride", 2), ("z_stride", 2), ("B_stride", 3), ("C_stride", 3))]
-        + [(n, c_void_p) for n in ("A", "D", "dt_bias", "state_in", "lengths", "out")] + [("out_stride", c_int64 * 2)]
-        + [(n, c_void_p) for n in ("state_out", "kept", "dout")] + [("dout_stride", c_int64 * 2)]
+        + [(n, c_int64) for n in ("u_b", "u_t", "dt_b", "dt_t", "z_b", "z_t", "B_b", "B_t", "B_g", "C_b", "C_t", "C_g")]
+        + [(n, c_void_p) for n in ("A", "D", "dt_bias", "state_in", "lengths", "out")] + [("out_b", c_int64), ("out_t", c_int64)]
+        + [(n, c_void_p) for n in ("state_out", "kept", "dout")] + [("dout_b", c_int64), ("dout_t", c_int64)]
         + [(n, c_void_p) for n in ("du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias")])
 
 
@@ -259,6 +259,7 @@ PROTOTYPES = {
 }
 
 _lib = None
+_torch = None
 
 
 def lib():
@@ -310,14 +311,18 @@ def stream_ptr():
 def launch_on(device, name, *args):
     """Call the entry point `name` with the current stream of `device` -- which need not be the current device -- behind its
     arguments, and check its status."""
-    import torch
+    global _torch
+    if _torch is None:
+        import torch
+        torch.cuda.init()
+        _torch = torch
     index = device.index
-    fn = getattr(lib(), name)
-    if torch.cuda.current_device() == index:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    fn = getattr(_lib or lib(), name)
+    if _torch._C._cuda_getDevice() == index:
+        status = fn(*args, _torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        with _torch.cuda.device(index):
+            status = fn(*args, _torch._C._cuda_getCurrentRawStream(index))
     if status != AVSI_OK:
         check(status, name)
 

@@ -7,9 +7,11 @@
 // and gradients are zero, and nothing is read.
 //
 // All of it is bound by memory: one read of x (and dy), one write.  A thread owns 16 bytes of channels and a run of consecutive
-// time steps, whose window slides through its registers, so an input is read once per run and K - 1 inputs again at its start.  In
-// the backward pass the run is followed by K - 1 steps of the next one (dx needs their dpre); the weights' gradients stay in
-// registers over all runs of a thread, are added over a workgroup in LDS and over the workgroups by a second launch, in a fixed order.
+// time steps, which it takes four at a time: the loads of the next four are in flight while these are computed, and the K - 1 inputs in
+// front of them stay in registers, so an input is read once per run and K - 1 inputs again at its start.  In the backward pass the
+// run is followed by K - 1 steps of the next one (dx needs their dpre); the weights' gradients stay in registers over all runs of a
+// thread, are added over a workgroup in LDS and over the workgroups by a second launch, in a fixed order.
+// Channels in no whole pieces: the last thread takes the last whole piece, which overlaps its neighbour's; both write the same values.
 #include "avsi_common.h"
 #include "avsi_wave.h"
 
@@ -33,155 +35,220 @@ __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int T) {
     return n < 0 ? 0 : (n < T ? n : T);
 }
 
-// Input t of the sequence, t >= 1 - K: from the state where t < 0.
-template <typename T, int K, int V>
-__device__ __forceinline__ void input(const Conv& a, const T* xb, int b, int t, int c, int n, float (&f)[V]) {
-    if (t >= 0) {
-        avsi_load<T, V>(xb + (int64_t)t * a.xt + c, n, f);
-    } else if (a.state) {
-        avsi_load<T, V>((const T*)a.state + ((int64_t)b * (K - 1) + K - 1 + t) * a.D + c, n, f);
-    } else {
+// A thread's channels c .. c + V - 1; SMALL: fewer channels than V exist, and they go one by one.
+template <typename T, int V, bool SMALL> struct Lane {
+    int c;
+    __device__ __forceinline__ Lane(int piece, int D) { c = SMALL ? 0 : (piece * V < D - V ? piece * V : D - V); }
+    __device__ __forceinline__ void load(const T* row, int D, avsi_pack<T, V>& v) const {
+        if (!SMALL) {
+            v.load(row + c);
+        } else {
+            float f[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = 0.f;
+            for (int i = 0; i < V; ++i) f[i] = (float)row[i < D ? i : D - 1];
+            v.set(f);
+        }
+    }
+    __device__ __forceinline__ void store(T* row, int D, const avsi_pack<T, V>& v) const {
+        if (!SMALL) {
+            v.store(row + c);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < D) row[i] = (T)v.at(i);
+        }
+    }
+    __device__ __forceinline__ void store(T* row, int D, const float (&f)[V]) const {
+        avsi_pack<T, V> v;
+        v.set(f);
+        store(row, D, v);
+    }
+    __device__ __forceinline__ int channel(int i, int D) const { return SMALL ? (i < D ? i : D - 1) : c + i; }
+};
+
+// Input t of the sequence, 1 - K <= t < 0: from the state, if there is one.
+template <typename T, int K, int V, bool SMALL>
+__device__ __forceinline__ void early(const Conv& a, const Lane<T, V, SMALL>& at, int64_t b, int t, float (&f)[V]) {
+    avsi_pack<T, V> v;
+    if (a.state) at.load((const T*)a.state + (b * (K - 1) + K - 1 + t) * a.D, a.D, v);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = a.state ? v.at(i) : 0.f;
+}
+// The K - 1 inputs in front of t0 into x[0 .. K - 2].
+template <typename T, int K, int V, int N, bool SMALL>
+__device__ __forceinline__ void history(const Conv& a, const Lane<T, V, SMALL>& at, const T* xb, int64_t b, int t0, float (&x)[N][V]) {
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+        const int t = t0 - K + 1 + k;
+        if (t >= 0) {
+            avsi_pack<T, V> v;
+            at.load(xb + (int64_t)t * a.xt, a.D, v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[k][i] = v.at(i);
+        } else {
+            early<T, K, V, SMALL>(a, at, b, t, x[k]);
+        }
     }
 }
 
-template <typename T, int K, int V>
-__device__ __forceinline__ void weights(const Conv& a, int c, int n, float (&w)[K][V], float (&bias)[V]) {
+template <typename T, int K, int V, bool SMALL>
+__device__ __forceinline__ void weights(const Conv& a, const Lane<T, V, SMALL>& at, float (&w)[K][V], float (&bias)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+        const int c = at.channel(i, a.D);
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k][i] = i < n ? a.w[(int64_t)(c + i) * K + k] : 0.f;
-        bias[i] = a.bias && i < n ? a.bias[c + i] : 0.f;
+        for (int k = 0; k < K; ++k) w[k][i] = a.w[(int64_t)c * K + k];
+        bias[i] = a.bias ? a.bias[c] : 0.f;
     }
 }
 
-template <typename T, int K> __global__ __launch_bounds__(256) void conv_fwd_kernel(Conv a, int runs) {
+template <typename T, int K, bool SMALL> __global__ __launch_bounds__(256) void conv_fwd_kernel(Conv a, int runs) {
     constexpr int V = channels<T, K>();
     const int nv = (a.D + V - 1) / V;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int c = (int)(id % nv) * V;
-    const int64_t rest = id / nv;
-    const int b = (int)(rest / runs), t0 = (int)(rest % runs) * a.run;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, rest = id / nv, b = rest / runs;
+    const Lane<T, V, SMALL> at((int)(id % nv), a.D);
+    const int t0 = (int)(rest % runs) * a.run;
     if (b >= a.B) return;
-    const int n = a.D - c, len = length_of(a.lengths, b, a.T);
+    const int len = length_of(a.lengths, (int)b, a.T);
     const int t1 = t0 + a.run < a.T ? t0 + a.run : a.T, live = len < t1 ? len : t1;
-    const T* xb = (const T*)a.x + (int64_t)b * a.xb;
-    T* yb = (T*)a.y + (int64_t)b * a.yb + c;
-    float w[K][V], bias[V], win[K][V], nx[V];
+    const T* xb = (const T*)a.x + b * a.xb;
+    T* yb = (T*)a.y + b * a.yb;
+    float x[K + 3][V];
     if (t0 < live) {
-        weights<T, K, V>(a, c, n, w, bias);
+        float w[K][V], bias[V];
+        avsi_pack<T, V> next[4];
+        auto load = [&](int t) {
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) input<T, K, V>(a, xb, b, t0 - K + 1 + k, c, n, win[k + 1]);
-        avsi_load<T, V>(xb + (int64_t)t0 * a.xt + c, n, nx);
-    }
-    for (int t = t0; t < live; ++t) {
-        float o[V];
+            for (int j = 0; j < 4; ++j) at.load(xb + (int64_t)(t + j < live ? t + j : live - 1) * a.xt, a.D, next[j]);
+        };
+        load(t0);
+        weights<T, K, V, SMALL>(a, at, w, bias);
+        history<T, K, V, K + 3, SMALL>(a, at, xb, b, t0, x);
+        for (int t = t0; t < live; t += 4) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k) win[k][i] = win[k + 1][i];
-            win[K - 1][i] = nx[i];
+                for (int i = 0; i < V; ++i) x[K - 1 + j][i] = next[j].at(i);
+            load(t + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float p = bias[i];
+#pragma unroll
+                    for (int k = 0; k < K; ++k) p = fmaf(w[k][i], x[j + k][i], p);
+                    const float s = p * avsi_sigmoid(p);
+                    o[i] = a.silu ? s : p;
+                }
+                if (t + j < live) at.store(yb + (int64_t)(t + j) * a.yt, a.D, o);
+            }
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[k][i] = x[k + 4][i];
         }
-        if (t + 1 < live) avsi_load<T, V>(xb + (int64_t)(t + 1) * a.xt + c, n, nx);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float p = bias[i];
-#pragma unroll
-            for (int k = 0; k < K; ++k) p = fmaf(w[k][i], win[k][i], p);
-            o[i] = a.silu ? p * avsi_sigmoid(p) : p;
-        }
-        avsi_store<T, V>(yb + (int64_t)t * a.yt, n, o);
     }
     float zero[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) zero[i] = 0.f;
-    for (int t = live > t0 ? live : t0; t < t1; ++t) avsi_store<T, V>(yb + (int64_t)t * a.yt, n, zero);
+    for (int t = live > t0 ? live : t0; t < t1; ++t) at.store(yb + (int64_t)t * a.yt, a.D, zero);
     if (a.state_out && t0 == 0) {        // the last K - 1 inputs in front of `len`
+        history<T, K, V, K + 3, SMALL>(a, at, xb, b, len, x);
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) {
-            input<T, K, V>(a, xb, b, len - K + 1 + k, c, n, nx);
-            avsi_store<T, V>((T*)a.state_out + ((int64_t)b * (K - 1) + k) * a.D + c, n, nx);
-        }
+        for (int k = 0; k < K - 1; ++k) at.store((T*)a.state_out + (b * (K - 1) + k) * a.D, a.D, x[k]);
     }
 }
 
 // part: [gridDim.y][K + 1][D].  A workgroup: `wide` threads along the channels (a power of two), 256 / wide runs.
-template <typename T, int K> __global__ __launch_bounds__(256) void conv_bwd_kernel(Conv a, int runs, int wide, float* __restrict__ part) {
+template <typename T, int K, bool SMALL>
+__global__ __launch_bounds__(256) void conv_bwd_kernel(Conv a, int runs, int wide, float* __restrict__ part) {
     constexpr int V = channels<T, K>();
     __shared__ float lds[256 * V];
-    const int lane = threadIdx.x % wide, slot = threadIdx.x / wide, slots = 256 / wide;
-    const int c = (blockIdx.x * wide + lane) * V, n = a.D - c;
+    const int piece = blockIdx.x * wide + threadIdx.x % wide, slot = threadIdx.x / wide, slots = 256 / wide;
+    const bool mine = piece * V < a.D;
+    const Lane<T, V, SMALL> at(piece, a.D);
     float w[K][V], bias[V], dw[K][V], db[V];
-    weights<T, K, V>(a, c, n, w, bias);
+    weights<T, K, V, SMALL>(a, at, w, bias);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         db[i] = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k) dw[k][i] = 0.f;
     }
-    if (n > 0)
+    if (mine)
         for (int64_t r = (int64_t)blockIdx.y * slots + slot; r < (int64_t)a.B * runs; r += (int64_t)gridDim.y * slots) {
-            const int b = (int)(r / runs), t0 = (int)(r % runs) * a.run, len = length_of(a.lengths, b, a.T);
+            const int64_t b = r / runs;
+            const int t0 = (int)(r % runs) * a.run, len = length_of(a.lengths, (int)b, a.T);
             const int t1 = t0 + a.run < a.T ? t0 + a.run : a.T;
-            const T* xb = (const T*)a.x + (int64_t)b * a.xb;
-            const T* gb = (const T*)a.dy + (int64_t)b * a.gb + c;
-            T* dxb = (T*)a.y + (int64_t)b * a.yb + c;
-            float win[K][V], dp[K][V], nx[V], ng[V];
+            const T* xb = (const T*)a.x + b * a.xb;
+            const T* gb = (const T*)a.dy + b * a.gb;
+            T* dxb = (T*)a.y + b * a.yb;
+            // x[K - 1 + j] and d[K - 1 + j] are input and dpre of step t + j; dx[t - K + 1 + j] is complete with d[j .. j + K - 1]
+            float x[K + 3][V], d[K + 3][V];
 #pragma unroll
-            for (int i = 0; i < V; ++i)
+            for (int k = 0; k < K - 1; ++k)
 #pragma unroll
-                for (int k = 0; k < K; ++k) dp[k][i] = win[k][i] = 0.f;
+                for (int i = 0; i < V; ++i) d[k][i] = 0.f;
             if (t0 < len) {
+                const int stop = len < t1 + K - 1 ? len : t1 + K - 1;       // steps that are read
+                avsi_pack<T, V> nx[4], ng[4];
+                auto load = [&](int t) {
 #pragma unroll
-                for (int k = 0; k < K - 1; ++k) input<T, K, V>(a, xb, b, t0 - K + 1 + k, c, n, win[k + 1]);
-                avsi_load<T, V>(xb + (int64_t)t0 * a.xt + c, n, nx);
-                avsi_load<T, V>(gb + (int64_t)t0 * a.gt, n, ng);
-            }
-            // dp[j] is dpre[t - K + 1 + j]; from t = t0 + K - 1 on dx[t - K + 1] is complete
-            for (int t = t0; t < t1 + K - 1; ++t) {
-                const bool live = t < len;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-#pragma unroll
-                    for (int k = 0; k < K - 1; ++k) {
-                        win[k][i] = win[k + 1][i];
-                        dp[k][i] = dp[k + 1][i];
+                    for (int j = 0; j < 4; ++j) {
+                        const int64_t u = t + j < stop ? t + j : stop - 1;
+                        at.load(xb + u * a.xt, a.D, nx[j]);
+                        at.load(gb + u * a.gt, a.D, ng[j]);
                     }
-                    win[K - 1][i] = live ? nx[i] : 0.f;
-                    float p = bias[i];
+                };
+                load(t0);
+                history<T, K, V, K + 3, SMALL>(a, at, xb, b, t0, x);
+                for (int t = t0; t < t1 + K - 1; t += 4) {
+                    float g[4][V];
 #pragma unroll
-                    for (int k = 0; k < K; ++k) p = fmaf(w[k][i], win[k][i], p);
-                    float slope = 1.f;
-                    if (a.silu) {
-                        const float s = avsi_sigmoid(p);
-                        slope = s * fmaf(p, 1.f - s, 1.f);
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            x[K - 1 + j][i] = nx[j].at(i);
+                            g[j][i] = ng[j].at(i);
+                        }
+                    load(t + 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool live = t + j < stop, own = t + j < t1 && live;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            float p = bias[i];
+#pragma unroll
+                            for (int k = 0; k < K; ++k) p = fmaf(w[k][i], x[j + k][i], p);
+                            const float s = avsi_sigmoid(p), slope = s * fmaf(p, 1.f - s, 1.f);
+                            const float e = live ? g[j][i] * (a.silu ? slope : 1.f) : 0.f, mineonly = own ? e : 0.f;
+                            d[K - 1 + j][i] = e;
+                            db[i] += mineonly;
+#pragma unroll
+                            for (int k = 0; k < K; ++k) dw[k][i] = fmaf(mineonly, x[j + k][i], dw[k][i]);
+                        }
+                        float o[V];
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            float s = 0.f;
+#pragma unroll
+                            for (int k = 0; k < K; ++k) s = fmaf(w[K - 1 - k][i], d[j + k][i], s);
+                            o[i] = s;
+                        }
+                        const int u = t + j - K + 1;
+                        if (u >= t0 && u < t1) at.store(dxb + (int64_t)u * a.yt, a.D, o);
                     }
-                    dp[K - 1][i] = live ? ng[i] * slope : 0.f;
-                }
-                if (t + 1 < len && t + 1 < t1 + K - 1) {
-                    avsi_load<T, V>(xb + (int64_t)(t + 1) * a.xt + c, n, nx);
-                    avsi_load<T, V>(gb + (int64_t)(t + 1) * a.gt, n, ng);
-                }
-                if (t < t1) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        db[i] += dp[K - 1][i];
+                    for (int k = 0; k < K - 1; ++k)
 #pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][i] = fmaf(dp[K - 1][i], win[k][i], dw[k][i]);
-                    }
+                        for (int i = 0; i < V; ++i) {
+                            x[k][i] = x[k + 4][i];
+                            d[k][i] = d[k + 4][i];
+                        }
                 }
-                if (t - K + 1 >= t0) {
-                    float o[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        float s = 0.f;
-#pragma unroll
-                        for (int k = 0; k < K; ++k) s = fmaf(w[K - 1 - k][i], dp[k][i], s);
-                        o[i] = s;
-                    }
-                    avsi_store<T, V>(dxb + (int64_t)(t - K + 1) * a.yt, n, o);
-                }
+            } else {
+                for (int t = t0; t < t1; ++t) at.store(dxb + (int64_t)t * a.yt, a.D, d[0]);
             }
         }
     if (!part) return;
@@ -192,10 +259,11 @@ template <typename T, int K> __global__ __launch_bounds__(256) void conv_bwd_ker
         for (int i = 0; i < V; ++i) lds[threadIdx.x * V + i] = k < K ? dw[k < K ? k : 0][i] : db[i];
         __syncthreads();
         for (int i = threadIdx.x; i < wide * V; i += 256) {
-            const int at = blockIdx.x * wide * V + i;
+            const int of = blockIdx.x * wide + i / V;
+            const int c = Lane<T, V, SMALL>(of, a.D).c + i % V;
             float s = 0.f;
             for (int j = 0; j < slots; ++j) s += lds[j * wide * V + i];
-            if (at < a.D) part[((int64_t)blockIdx.y * (K + 1) + k) * a.D + at] = s;
+            if (of * V < a.D && c < a.D) part[((int64_t)blockIdx.y * (K + 1) + k) * a.D + c] = s;
         }
     }
 }
@@ -215,41 +283,60 @@ __global__ __launch_bounds__(1024) void conv_wgrad_sum_kernel(const float* __res
 template <typename T, int K> __global__ __launch_bounds__(256) void conv_step_kernel(Conv a) {
     constexpr int V = channels<T, K>();
     const int nv = (a.D + V - 1) / V;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int c = (int)(id % nv) * V;
-    const int64_t b = id / nv;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, b = id / nv;
     if (b >= a.B) return;
-    const int n = a.D - c;
+    // (no overlap here, where state is read and written: the thread that the last channel cuts goes one by one)
+    const int c = (int)(id % nv) * V, n = a.D - c;
     T* st = (T*)a.state_out + b * (K - 1) * a.D + c;
-    avsi_raw<T, V> win[K];
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k) win[k] = avsi_load_raw<T, V>(st + (int64_t)k * a.D, n);
-    win[K - 1] = avsi_load_raw<T, V>((const T*)a.x + b * a.xb + c, n);
-    float w[K][V], bias[V], o[V];
-    weights<T, K, V>(a, c, n, w, bias);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        float p = bias[i];
-#pragma unroll
-        for (int k = 0; k < K; ++k) p = fmaf(w[k][i], (float)win[k].v[i], p);
-        o[i] = a.silu ? p * avsi_sigmoid(p) : p;
-    }
-    avsi_store<T, V>((T*)a.y + b * a.yb + c, n, o);
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k) {
+    const T* x = (const T*)a.x + b * a.xb + c;
+    avsi_pack<T, V> win[K];
+    auto fetch = [&](const T* p, avsi_pack<T, V>& v) {
         float f[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = (float)win[k + 1].v[i];
-        avsi_store<T, V>(st + (int64_t)k * a.D, n, f);
+        for (int i = 0; i < V; ++i) f[i] = (float)p[i < n ? i : n - 1];
+        v.set(f);
+    };
+    if (n >= V) {
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) win[k].load(st + (int64_t)k * a.D);
+        win[K - 1].load(x);
+    } else {
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) fetch(st + (int64_t)k * a.D, win[k]);
+        fetch(x, win[K - 1]);
+    }
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int ch = c + (i < n ? i : n - 1);
+        float p = a.bias ? a.bias[ch] : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) p = fmaf(a.w[(int64_t)ch * K + k], win[k].at(i), p);
+        const float s = p * avsi_sigmoid(p);
+        o[i] = a.silu ? s : p;
+    }
+    T* y = (T*)a.y + b * a.yb + c;
+    if (n >= V) {
+        avsi_pack<T, V> v;
+        v.set(o);
+        v.store(y);
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) win[k + 1].store(st + (int64_t)k * a.D);
+    } else {
+        for (int i = 0; i < n; ++i) {
+            y[i] = (T)o[i];
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k) st[(int64_t)k * a.D + i] = (T)win[k + 1].at(i);
+        }
     }
 }
 
 int channels_of(int dtype, int taps) { return dtype == AVSI_F32 || taps > 4 ? 4 : 8; }
 int vectors(int D, int dtype, int taps) { return (int)avsi_ceil_div(D, channels_of(dtype, taps)); }
 
-// Steps per run: 4 .. 32, the longest that leaves 2^17 threads (2 waves per SIMD).
+// Steps per run, a multiple of four: 4 .. 32, the longest that leaves 2^17 threads (2 waves per SIMD).
 int run_length(int64_t B, int T, int D, int dtype, int taps) {
-    int64_t r = B * T * vectors(D, dtype, taps) >> 17;
+    const int64_t r = (B * T * vectors(D, dtype, taps) >> 17) / 4 * 4;
     return (int)(r < 4 ? 4 : r > 32 ? 32 : r);
 }
 
@@ -267,16 +354,20 @@ bool shape_ok(int dtype, int B, int T, int D, int taps) { return avsi_dtype_ok(d
 
 }  // namespace
 
-#define AVSI_CONV_K(T, GO)        \
-    switch (taps) {               \
-        case 2: GO(T, 2); break;  \
-        case 3: GO(T, 3); break;  \
-        case 4: GO(T, 4); break;  \
-        case 5: GO(T, 5); break;  \
-        case 6: GO(T, 6); break;  \
-        case 7: GO(T, 7); break;  \
-        default: GO(T, 8); break; \
+#define AVSI_CONV_K(T, GO)                                \
+    if (dim < channels_of(dtype, taps)) {                 \
+        switch (taps) { AVSI_CONV_TAPS(T, GO, true) }     \
+    } else {                                              \
+        switch (taps) { AVSI_CONV_TAPS(T, GO, false) }    \
     }
+#define AVSI_CONV_TAPS(T, GO, SMALL) \
+    case 2: GO(T, 2, SMALL); break;  \
+    case 3: GO(T, 3, SMALL); break;  \
+    case 4: GO(T, 4, SMALL); break;  \
+    case 5: GO(T, 5, SMALL); break;  \
+    case 6: GO(T, 6, SMALL); break;  \
+    case 7: GO(T, 7, SMALL); break;  \
+    default: GO(T, 8, SMALL); break;
 #define AVSI_CONV_T(GO)                                         \
     if (dtype == AVSI_F32) { AVSI_CONV_K(float, GO) }           \
     else if (dtype == AVSI_BF16) { AVSI_CONV_K(__bf16, GO) }    \
@@ -291,7 +382,7 @@ extern "C" int avsi_causal_conv(const void* x, int64_t x_stride_b, int64_t x_str
     if (wgs > 0x7fffffff) return AVSI_ERR_UNSUPPORTED;
     Conv a = {x, nullptr, state, y, state_out, w, bias, lengths, x_stride_b, x_stride_t, y_stride_b, y_stride_t, 0, 0, batch, time, dim, silu, run};
     avsi_clear_error();
-#define AVSI_GO(T, K) hipLaunchKernelGGL((conv_fwd_kernel<T, K>), dim3(wgs), dim3(256), 0, (hipStream_t)stream, a, runs)
+#define AVSI_GO(T, K, SMALL) hipLaunchKernelGGL((conv_fwd_kernel<T, K, SMALL>), dim3(wgs), dim3(256), 0, (hipStream_t)stream, a, runs)
     AVSI_CONV_T(AVSI_GO)
 #undef AVSI_GO
     return avsi_launch_status();
@@ -319,7 +410,7 @@ extern "C" int avsi_causal_conv_bwd(const void* dy, int64_t dy_stride_b, int64_t
     const dim3 grid(avsi_ceil_div(vectors(dim, dtype, taps), wide), groups);
     float* part = dw ? (float*)workspace : nullptr;
     avsi_clear_error();
-#define AVSI_GO(T, K) hipLaunchKernelGGL((conv_bwd_kernel<T, K>), grid, dim3(256), 0, (hipStream_t)stream, a, runs, wide, part)
+#define AVSI_GO(T, K, SMALL) hipLaunchKernelGGL((conv_bwd_kernel<T, K, SMALL>), grid, dim3(256), 0, (hipStream_t)stream, a, runs, wide, part)
     AVSI_CONV_T(AVSI_GO)
 #undef AVSI_GO
     if (dw)
@@ -335,7 +426,7 @@ extern "C" int avsi_causal_conv_step(const void* x, int64_t x_stride_b, int dtyp
     const int64_t wgs = avsi_ceil_div((int64_t)batch * vectors(dim, dtype, taps), 256);
     if (wgs > 0x7fffffff) return AVSI_ERR_UNSUPPORTED;
     avsi_clear_error();
-#define AVSI_GO(T, K) hipLaunchKernelGGL((conv_step_kernel<T, K>), dim3(wgs), dim3(256), 0, (hipStream_t)stream, a)
+#define AVSI_GO(T, K, SMALL) hipLaunchKernelGGL((conv_step_kernel<T, K>), dim3(wgs), dim3(256), 0, (hipStream_t)stream, a)
     AVSI_CONV_T(AVSI_GO)
 #undef AVSI_GO
     return avsi_launch_status();

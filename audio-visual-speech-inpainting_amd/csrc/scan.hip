@@ -546,14 +546,26 @@ template <bool BACK> __global__ __launch_bounds__(256) void scan_join_kernel(Sca
         A[j] = n < p.N ? p.A[(int64_t)d * p.N + n] * LOG2E : 0.f;
         h[j] = !BACK && p.state && n < p.N ? p.state[((int64_t)b * p.dim + d) * p.N + n] : 0.f;
     }
-    for (int i = 1; i < p.chunks; ++i) {
-        const int64_t lead = (int64_t)b * p.chunks + (BACK ? p.chunks - 1 - i : i);
-        avsi_f4* e = (avsi_f4*)(p.ends + ((lead * p.dim + d) * QB + ql) * 4);
-        const float s = p.sums[lead * p.dim + d];
-        avsi_f4 v = *e;
+    // (the rows do not depend on each other: eight of them in flight)
+    for (int i0 = 1; i0 < p.chunks; i0 += 8) {
+        avsi_f4 v[8];
+        float sum[8];
+        auto row = [&](int i) {
+            i = i < p.chunks ? i : p.chunks - 1;
+            return ((int64_t)b * p.chunks + (BACK ? p.chunks - 1 - i : i)) * p.dim + d;
+        };
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = h[j] = fmaf(__builtin_amdgcn_exp2f(s * A[j]), h[j], v[j]);
-        *e = v;
+        for (int k = 0; k < 8; ++k) {
+            v[k] = *(const avsi_f4*)(p.ends + (row(i0 + k) * QB + ql) * 4);
+            sum[k] = p.sums[row(i0 + k)];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (i0 + k < p.chunks) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[k][j] = h[j] = fmaf(__builtin_amdgcn_exp2f(sum[k] * A[j]), h[j], v[k][j]);
+                *(avsi_f4*)(p.ends + (row(i0 + k) * QB + ql) * 4) = v[k];
+            }
     }
 }
 
@@ -835,18 +847,29 @@ __global__ __launch_bounds__(1024) void scan_wgrad_sum_kernel(const float* __res
     }
 }
 
-// dB, dC [batch][time][groups][N] = sums over the blocks of part_bc; zero behind a length.
+// dB, dC [batch][time][groups][N] = sums over the blocks of part_bc; zero behind a length.  A thread: four states of one of the two,
+// the partials of eight blocks in flight.
 template <typename T> __global__ __launch_bounds__(256) void scan_bc_sum_kernel(Scan p, int NP, T* __restrict__ dB, T* __restrict__ dC) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, tokens = (int64_t)p.batch * p.T;
-    if (id >= tokens * p.groups * 2 * NP) return;
-    const int n = (int)(id % NP), which = (int)(id / NP % 2);
-    const int64_t tg = id / (2 * NP);
-    const int t = (int)(tg / p.groups % p.T), b = (int)(tg / p.groups / p.T);
+    const int Q = NP / 2;                   // quads of dB and dC of a token and group
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, tg = id / Q;
+    if (tg >= (int64_t)p.batch * p.T * p.groups) return;
+    const int q = (int)(id % Q), n = 4 * (q % (NP / 4)), t = (int)(tg / p.groups % p.T), b = (int)(tg / p.groups / p.T);
     if (n >= p.N) return;
-    float s = 0.f;
-    if (t < length_of(p.lengths, b, p.T))
-        for (int k = 0; k < p.blocks; ++k) s += p.part_bc[(tg * p.blocks + k) * 2 * NP + which * NP + n];
-    (which ? dC : dB)[tg * p.N + n] = (T)s;
+    avsi_f4 s = {0.f, 0.f, 0.f, 0.f};
+    if (t < length_of(p.lengths, b, p.T)) {
+        const avsi_f4* at = (const avsi_f4*)p.part_bc + tg * p.blocks * Q + q;
+        int k = 0;
+        for (; k + 8 <= p.blocks; k += 8) {
+            avsi_f4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = at[(int64_t)(k + i) * Q];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
+        for (; k < p.blocks; ++k) s += at[(int64_t)k * Q];
+    }
+    const float f[4] = {s[0], s[1], s[2], s[3]};
+    put_quad<T>((q < NP / 4 ? dB : dC) + tg * p.N + n, p.N - n, f);
 }
 
 // ---------------------------------------------------------------------------------------------------------- one token
@@ -1038,7 +1061,7 @@ extern "C" int avsi_selective_scan_bwd(const avsi_scan_args* a, void* workspace,
     hipStream_t s = (hipStream_t)stream;
     avsi_clear_error();
     AVSI_SCAN_T(AVSI_SCAN_N, go_bwd)
-    const int64_t bc = (int64_t)p.batch * p.T * p.groups * 2 * NP;
+    const int64_t bc = (int64_t)p.batch * p.T * p.groups * NP / 2;
     const dim3 grid(avsi_ceil_div(bc, 256));
     if (a->dtype == AVSI_F32)
         hipLaunchKernelGGL((scan_bc_sum_kernel<float>), grid, dim3(256), 0, s, p, NP, (float*)a->dB, (float*)a->dC);

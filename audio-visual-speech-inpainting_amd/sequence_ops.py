@@ -19,11 +19,11 @@ def _device(what, first, *others):
     """The device of the operands; all of them have to be on it."""
     if not first.is_cuda:
         _lib.require_cuda(first)
-    dev = first.device
+    index = first.get_device()
     for t in others:
-        if t is not None and t.device != dev:
-            _bad("%s: operands on %s and %s", what, dev, t.device)
-    return dev
+        if t is not None and t.get_device() != index:
+            _bad("%s: operands on %s and %s", what, first.device, t.device)
+    return first.device
 
 
 def _p(t):
@@ -32,13 +32,10 @@ def _p(t):
 
 def _overlap(a, b):
     """Whether two tensors share memory (by the span of their elements)."""
-    def span(t):
-        if not t.numel():
-            return 0, 0
-        lo = t.data_ptr()
-        return lo, lo + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    lo, hi = a.data_ptr(), b.data_ptr()
+    if lo > hi:
+        a, b, lo, hi = b, a, hi, lo
+    return bool(a.numel() and b.numel()) and hi < lo + (1 + sum((n - 1) * s for n, s in zip(a.shape, a.stride()))) * a.element_size()
 
 
 # ------------------------------------------------------------------------------------------------------------- layer norm
@@ -91,14 +88,14 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, y=None):
             _bad("layer_norm: y must have x's shape and type and memory of its own")
     dev = _device("layer_norm", x, gamma, beta, y)
     if y is None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((2, M), dtype=torch.float32, device=dev)
+        y = x.new_empty(x.shape)
+    stats = x.new_empty((2, M), dtype=torch.float32)
     if M:
         w = gamma if gamma is not None else beta
         p = stats.data_ptr()
         _lib.launch_on(dev, "avsi_layer_norm", x.data_ptr(), xs, _CODES[x.dtype], _p(gamma), _p(beta), 0 if w is None else _CODES[w.dtype],
                        y.data_ptr(), ys, p, p + 4 * M, M, C, eps)
-    return y, stats[0], stats[1]
+    return (y, *stats.unbind(0))
 
 
 def layer_norm_bwd(dy, x, mean, rstd, gamma=None, want_wgrad=True, dx=None):
@@ -120,11 +117,11 @@ def layer_norm_bwd(dy, x, mean, rstd, gamma=None, want_wgrad=True, dx=None):
             _bad("layer_norm_bwd: dx must have x's shape and type and memory of its own")
     dev = _device("layer_norm_bwd", dy, x, mean, rstd, gamma, dx)
     if dx is None:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dx = x.new_empty(x.shape)
     code = _CODES[x.dtype]
     grads, ws, nbytes = None, None, 0
     if want_wgrad:
-        grads = torch.empty((2, C), dtype=torch.float32, device=dev)
+        grads = x.new_empty((2, C), dtype=torch.float32)
         if not M:
             grads.zero_()
     if M:
@@ -135,7 +132,7 @@ def layer_norm_bwd(dy, x, mean, rstd, gamma=None, want_wgrad=True, dx=None):
         _lib.launch_on(dev, "avsi_layer_norm_bwd", dy.data_ptr(), dys, x.data_ptr(), xs, code, mean.data_ptr(), rstd.data_ptr(), _p(gamma),
                        0 if gamma is None else _CODES[gamma.dtype], dx.data_ptr(), dxs, p, None if p is None else p + 4 * C, M, C, _p(ws),
                        nbytes)
-    return (dx, grads[0], grads[1]) if want_wgrad else (dx, None, None)
+    return (dx, *grads.unbind(0)) if want_wgrad else (dx, None, None)
 
 
 # -------------------------------------------------------------------------------------------------------- causal convolution
@@ -150,12 +147,12 @@ def _seq(what, name, t, shape, dtype):
 
 def _vector(what, name, t, *shape):
     """A contiguous float32 weight."""
-    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
+    if t is not None and (t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous()):
         _bad("%s: %s must be contiguous float32 of shape %s", what, name, shape)
 
 
 def _state(what, t, shape, dtype):
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous()):
+    if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
         _bad("%s: state must be contiguous %s of shape %s", what, dtype, shape)
 
 
@@ -234,7 +231,7 @@ def causal_conv_step(x, w, bias=None, silu=True, *, state):
     if _overlap(x, state):
         _bad("causal_conv_step: x must not be part of the state")
     dev = _device("causal_conv_step", x, w, bias, state)
-    y = torch.empty((B, D), dtype=x.dtype, device=dev)
+    y = x.new_empty((B, D))
     if B:
         _lib.launch_on(dev, "avsi_causal_conv_step", x.data_ptr(), x.stride(0), _CODES[x.dtype], w.data_ptr(), _p(bias), int(silu),
                        state.data_ptr(), y.data_ptr(), D, B, D, K)
@@ -243,47 +240,48 @@ def causal_conv_step(x, w, bias=None, silu=True, *, state):
 
 # ------------------------------------------------------------------------------------------------------------ selective scan
 def _groups(what, name, t, lead, N, dtype):
-    """(groups, strides) of B or C: [..., groups, state], or [..., state] for one group."""
-    n = len(lead)
-    if t.dtype != dtype or t.dim() not in (n + 1, n + 2) or tuple(t.shape[:n]) != lead or t.shape[-1] != N:
-        _bad("%s: %s must be %s of shape %s + [groups, %d]", what, name, dtype, lead, N)
-    if N > 1 and t.stride(-1) != 1:
+    """(groups, strides of batch, time and group) of B or C: [..., groups, state], or [..., state] for one group."""
+    n, shape, st = len(lead), t.shape, t.stride()
+    if t.dtype is not dtype or len(shape) - n not in (1, 2) or shape[:n] != lead or shape[-1] != N:
+        _bad("%s: %s must be %s of shape %s + [groups, %d]", what, name, dtype, tuple(lead), N)
+    if N > 1 and st[-1] != 1:
         _bad("%s: %s must have unit stride along its states", what, name)
-    if t.dim() == n + 1:
-        return 1, (t.stride(0), t.stride(1) if n == 2 else 0, 0)
-    return t.shape[n], (t.stride(0), t.stride(1) if n == 2 else 0, t.stride(n))
+    one = len(shape) == n + 1
+    return 1 if one else shape[n], (st[0], st[1] if n == 2 else 0, 0 if one else st[n])
 
 
-def _scan_args(what, u, dt, A, B, C, D, z, dt_bias, softplus, lead):
-    """The checked operands that all forms of the scan take, as avsi_scan_args."""
-    if u.dtype not in _CODES or u.dim() != len(lead) + 1 or u.shape[-1] < 1:
-        _bad("%s: u must be a float32, bfloat16 or float16 tensor of %d dimensions", what, len(lead) + 1)
-    dim, dtype = u.shape[-1], u.dtype
+def _scan_operands(what, u, dt, A, B, C, D, z, dt_bias, softplus):
+    """The operands that all forms of the scan take, checked, as the leading fields of avsi_scan_args; u is [..., channels]."""
+    dtype, shape, su = u.dtype, u.shape, u.stride()
+    lead, dim, two = shape[:-1], shape[-1], len(shape) == 3
+    if dtype not in _CODES or dim < 1:
+        _bad("%s: u must be a float32, bfloat16 or float16 tensor with channels", what)
     if A.dim() != 2 or not 1 <= A.shape[1] <= 64:
         _bad("%s: A must be [channels, states] with 1 to 64 states", what)
     N = A.shape[1]
     _vector(what, "A", A, dim, N)
     _vector(what, "D", D, dim)
     _vector(what, "dt_bias", dt_bias, dim)
-    a = _lib.ScanArgs(_CODES[dtype], lead[0], lead[1] if len(lead) == 2 else 1, dim, N, 1, int(softplus))
     if lead[0] > 65535:
         _bad("%s: at most 65535 sequences", what)
-    for name, t in (("u", u), ("dt", dt), ("z", z)):
-        if t is None:
-            continue
-        if t.dtype != dtype or t.shape != u.shape:
-            _bad("%s: %s must be %s of shape %s, not %s of %s", what, name, dtype, tuple(u.shape), t.dtype, tuple(t.shape))
-        if dim > 1 and t.stride(-1) != 1:
-            _bad("%s: %s must have unit stride along its channels", what, name)
-        setattr(a, name, t.data_ptr())
-        s = getattr(a, name + "_stride")
-        s[0], s[1] = t.stride(0), t.stride(1) if len(lead) == 2 else 0
-    G, a.B_stride = _groups(what, "B", B, lead, N, dtype)
-    G2, a.C_stride = _groups(what, "C", C, lead, N, dtype)
+    if dt.dtype is not dtype or dt.shape != shape:
+        _bad("%s: dt must be %s of shape %s, not %s of %s", what, dtype, tuple(shape), dt.dtype, tuple(dt.shape))
+    sd = dt.stride()
+    if z is None:
+        sz = (0, 0, 1)
+    else:
+        if z.dtype is not dtype or z.shape != shape:
+            _bad("%s: z must be %s of shape %s, not %s of %s", what, dtype, tuple(shape), z.dtype, tuple(z.shape))
+        sz = z.stride()
+    if dim > 1 and not su[-1] == sd[-1] == sz[-1] == 1:
+        _bad("%s: u, dt and z must have unit stride along their channels", what)
+    G, sB = _groups(what, "B", B, lead, N, dtype)
+    G2, sC = _groups(what, "C", C, lead, N, dtype)
     if G != G2 or G < 1 or dim % G:
         _bad("%s: B and C must have one number of groups, which divides the %d channels", what, dim)
-    a.groups, a.B, a.C, a.A, a.D, a.dt_bias = G, B.data_ptr(), C.data_ptr(), A.data_ptr(), _p(D), _p(dt_bias)
-    return a, N
+    t = (lambda s: s[1]) if two else (lambda s: 0)
+    return N, (_CODES[dtype], lead[0], lead[1] if two else 1, dim, N, G, int(softplus), 0, u.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(),
+               C.data_ptr(), su[0], t(su), sd[0], t(sd), sz[0], t(sz), *sB, *sC, A.data_ptr(), _p(D), _p(dt_bias))
 
 
 def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, state=None, lengths=None, want_state=False, keep=False):
@@ -301,24 +299,24 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, 
     if u.dim() != 3:
         _bad("%s: u must be [batch, time, channels]", what)
     bsz, T, dim = u.shape
-    a, N = _scan_args(what, u, dt, A, B, C, D, z, dt_bias, softplus, (bsz, T))
+    N, operands = _scan_operands(what, u, dt, A, B, C, D, z, dt_bias, softplus)
     _state(what, state, (bsz, dim, N), torch.float32)
     _lengths(what, lengths, bsz)
     dev = _device(what, u, dt, A, B, C, D, z, dt_bias, state, lengths)
-    out = torch.empty((bsz, T, dim), dtype=u.dtype, device=dev)
-    new = torch.empty((bsz, dim, N), dtype=torch.float32, device=dev) if want_state else None
+    out = u.new_empty((bsz, T, dim))
+    new = A.new_empty((bsz, dim, N)) if want_state else None
     kept = None
     if not (bsz and T):
         if want_state and bsz:
             new.zero_() if state is None else new.copy_(state)
         return out, new, torch.empty(0, dtype=torch.float32, device=dev) if keep else None
     L = _lib.lib()
+    a = _lib.ScanArgs(*operands, _p(state), _p(lengths), out.data_ptr(), T * dim, dim, _p(new))
     if keep:
-        kept = torch.empty(L.avsi_selective_scan_kept_floats(a), dtype=torch.float32, device=dev)
-    a.state_in, a.lengths, a.out, a.state_out, a.kept = _p(state), _p(lengths), out.data_ptr(), _p(new), _p(kept)
-    a.out_stride[0], a.out_stride[1] = T * dim, dim
+        kept = A.new_empty(L.avsi_selective_scan_kept_floats(a))
+        a.kept = kept.data_ptr()
     nbytes = L.avsi_selective_scan_workspace_bytes(a)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
+    ws = A.new_empty(nbytes // 4) if nbytes else None
     _lib.launch_on(dev, "avsi_selective_scan", a, _p(ws), nbytes)
     return out, new, kept
 
@@ -331,11 +329,12 @@ def selective_scan_bwd(dout, u, dt, A, B, C, D=None, z=None, dt_bias=None, softp
     if u.dim() != 3:
         _bad("%s: u must be [batch, time, channels]", what)
     bsz, T, dim = u.shape
-    a, N = _scan_args(what, u, dt, A, B, C, D, z, dt_bias, softplus, (bsz, T))
-    a.dout_stride[0], a.dout_stride[1] = _seq(what, "dout", dout, (bsz, T, dim), u.dtype)
+    N, operands = _scan_operands(what, u, dt, A, B, C, D, z, dt_bias, softplus)
+    gb, gt = _seq(what, "dout", dout, (bsz, T, dim), u.dtype)
     _state(what, state, (bsz, dim, N), torch.float32)
     _lengths(what, lengths, bsz)
     L = _lib.lib()
+    a = _lib.ScanArgs(*operands)
     if kept.dtype != torch.float32 or not kept.is_contiguous() or kept.numel() != L.avsi_selective_scan_kept_floats(a):
         _bad("%s: kept must be what selective_scan returned with keep=True for these operands", what)
     dev = _device(what, u, dt, A, B, C, D, z, dt_bias, dout, kept, state, lengths)
@@ -346,7 +345,7 @@ def selective_scan_bwd(dout, u, dt, A, B, C, D=None, z=None, dt_bias=None, softp
     dD = None if D is None else torch.empty(dim, dtype=torch.float32, device=dev)
     ddt_bias = None if dt_bias is None else torch.empty(dim, dtype=torch.float32, device=dev)
     if bsz and T:
-        a.lengths, a.kept, a.dout = _p(lengths), kept.data_ptr(), dout.data_ptr()
+        a.lengths, a.kept, a.dout, a.dout_b, a.dout_t = _p(lengths), kept.data_ptr(), dout.data_ptr(), gb, gt
         a.du, a.ddt, a.dz, a.dB, a.dC = du.data_ptr(), ddt.data_ptr(), _p(dz), dB.data_ptr(), dC.data_ptr()
         a.dA, a.dD, a.ddt_bias = dA.data_ptr(), _p(dD), _p(ddt_bias)
         nbytes = L.avsi_selective_scan_bwd_workspace_bytes(a)
@@ -366,12 +365,11 @@ def selective_scan_step(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=T
     if u.dim() != 2:
         _bad("%s: u must be [batch, channels]", what)
     bsz, dim = u.shape
-    a, N = _scan_args(what, u, dt, A, B, C, D, z, dt_bias, softplus, (bsz,))
+    N, operands = _scan_operands(what, u, dt, A, B, C, D, z, dt_bias, softplus)
     _state(what, state, (bsz, dim, N), torch.float32)
     dev = _device(what, u, dt, A, B, C, D, z, dt_bias, state)
-    out = torch.empty((bsz, dim), dtype=u.dtype, device=dev)
+    out = u.new_empty((bsz, dim))
     if bsz:
-        a.out, a.state_out = out.data_ptr(), state.data_ptr()
-        a.out_stride[0] = dim
-        _lib.launch_on(dev, "avsi_selective_scan_step", a)
+        _lib.launch_on(dev, "avsi_selective_scan_step",
+                       _lib.ScanArgs(*operands, None, None, out.data_ptr(), dim, 0, state.data_ptr()))
     return out
