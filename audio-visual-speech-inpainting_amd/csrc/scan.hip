@@ -873,36 +873,62 @@ template <typename T> __global__ __launch_bounds__(256) void scan_bc_sum_kernel(
 }
 
 // ---------------------------------------------------------------------------------------------------------- one token
-template <typename T, int LN> __global__ __launch_bounds__(256) void scan_step_kernel(Scan p) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int ql = (int)(id % LN), d = (int)(id / LN % p.dim);
-    const int64_t b = id / LN / p.dim;
-    if (b >= p.batch) return;               // (whole groups of LN lanes leave: dim LN per sequence)
-    const int n0 = 4 * ql, n = p.N - n0, grp = d / (p.dim / p.groups);
-    float A[4], Bv[4], Cv[4], h[4];
-    avsi_load<float, 4>(p.A + (int64_t)d * p.N + n0, n, A);
-    avsi_load<T, 4>((const T*)p.B + b * p.Bb + grp * p.Bg + n0, n, Bv);
-    avsi_load<T, 4>((const T*)p.C + b * p.Cb + grp * p.Cg + n0, n, Cv);
-    float* st = p.state_out + (b * p.dim + d) * p.N + n0;
-    avsi_load<float, 4>(st, n, h);
-    const float u = (float)((const T*)p.u)[b * p.ub + d];
-    const float x = (float)((const T*)p.dt)[b * p.tb + d] + (p.bias ? p.bias[d] : 0.f);
-    const float delta = step_size(x, p.softplus), du = delta * u;
-    float y = 0.f;
+// Bound by the states, read and written once; a lane's four states of one channel over the sequences b, b + gridDim.y, ..., with the
+// next sequence's operands in flight.  EL: states in no whole quads, one by one.
+template <typename T, int LN, bool EL> __global__ __launch_bounds__(256) void scan_step_kernel(Scan p) {
+    const int id = blockIdx.x * 256 + threadIdx.x, ql = id % LN, d = id / LN, n0 = 4 * ql, left = p.N - n0;
+    if (d >= p.dim) return;                 // (whole groups of LN lanes leave)
+    const int grp = d / (p.dim / p.groups), c0 = n0 < p.N - 4 ? n0 : (p.N < 4 ? 0 : p.N - 4);    // (lanes without states read the last four)
+    float A[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        h[j] = fmaf(__builtin_amdgcn_exp2f(delta * (A[j] * LOG2E)), h[j], du * Bv[j]);
-        y = fmaf(h[j], Cv[j], y);
-    }
-    avsi_store<float, 4>(st, n, h);
-    y = avsi_group<LN>(y);
-    if (ql == 0) {
-        if (p.D) y = fmaf(p.D[d], u, y);
-        if (p.gated) {
-            const float z = (float)((const T*)p.z)[b * p.zb + d];
-            y *= z * avsi_sigmoid(z);
+    for (int j = 0; j < 4; ++j) A[j] = j < left ? p.A[(int64_t)d * p.N + n0 + j] * LOG2E : 0.f;
+    const float Dd = p.D ? p.D[d] : 0.f, bias = p.bias ? p.bias[d] : 0.f;
+    avsi_quad<T> Bq, Cq;
+    avsi_quad<float> hq;
+    T u, dt, z;
+    auto load = [&](int64_t b) {
+        const T* Bp = (const T*)p.B + b * p.Bb + grp * p.Bg;
+        const T* Cp = (const T*)p.C + b * p.Cb + grp * p.Cg;
+        const float* st = p.state_out + (b * p.dim + d) * p.N;
+        if (!EL) {
+            hq.load(st + c0);
+            Bq.load(Bp + c0);
+            Cq.load(Cp + c0);
+        } else {
+            float f[4], g[4], h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int n = n0 + j < p.N ? n0 + j : p.N - 1;
+                f[j] = (float)Bp[n], g[j] = (float)Cp[n], h[j] = st[n];
+            }
+            Bq.set(f), Cq.set(g), hq.set(h);
         }
-        ((T*)p.out)[b * p.ob + d] = (T)y;
+        u = ((const T*)p.u)[b * p.ub + d];
+        dt = ((const T*)p.dt)[b * p.tb + d];
+        z = ((const T*)p.z)[b * p.zb + d];
+    };
+    int64_t b = blockIdx.y;
+    load(b);
+    for (; b < p.batch; b += gridDim.y) {
+        float Bv[4], Cv[4], h[4];
+        Bq.get(Bv);
+        Cq.get(Cv);
+        hq.get(h);
+        const float uf = (float)u, x = (float)dt + bias, zf = (float)z;
+        load(b + gridDim.y < p.batch ? b + gridDim.y : b);       // (another sequence's states than those written below, or unused)
+        const float delta = step_size(x, p.softplus), du = delta * uf;
+        float y = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            h[j] = fmaf(__builtin_amdgcn_exp2f(delta * A[j]), h[j], du * Bv[j]);
+            y += j < left ? h[j] * Cv[j] : 0.f;
+        }
+        put_quad<float>(p.state_out + (b * p.dim + d) * p.N + n0, left, h);
+        y = avsi_group<LN>(y);
+        if (ql == 0) {
+            y = fmaf(Dd, uf, y);
+            ((T*)p.out)[b * p.ob + d] = (T)(p.gated ? y * (zf * avsi_sigmoid(zf)) : y);
+        }
     }
 }
 
@@ -931,7 +957,7 @@ void chunks_of(const avsi_scan_args* a, int* chunk, int* chunks) {
 }
 
 bool shape_ok(const avsi_scan_args* a) {
-    return a && avsi_dtype_ok(a->dtype) && a->batch > 0 && a->batch <= 65535 && a->time > 0 && a->dim > 0 && a->state > 0 &&
+    return a && avsi_dtype_ok(a->dtype) && a->batch > 0 && a->batch <= 65535 && a->time > 0 && a->dim > 0 && a->dim <= (1 << 26) && a->state > 0 &&
            a->groups > 0 && a->dim % a->groups == 0;
 }
 
@@ -984,7 +1010,11 @@ template <typename T, typename S> void go_bwd(const Scan& p, hipStream_t s) {
     hipLaunchKernelGGL((scan_bwd_kernel<T, S>), dim3(p.groups * p.blocks, p.chunks, p.batch), dim3(2 * S::NT), 0, s, p);
 }
 template <typename T, int LN> void go_step(const Scan& p, hipStream_t s) {
-    hipLaunchKernelGGL((scan_step_kernel<T, LN>), dim3(avsi_ceil_div((int64_t)p.batch * p.dim * LN, 256)), dim3(256), 0, s, p);
+    // as many workgroups as stay on the chip (eight a CU), each over several sequences
+    const int64_t along = avsi_ceil_div((int64_t)p.dim * LN, 256), most = avsi_ceil_div(8 * AVSI_NUM_CU, along);
+    const dim3 grid(along, p.batch < most ? p.batch : most);
+    if (p.N % 4) hipLaunchKernelGGL((scan_step_kernel<T, LN, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((scan_step_kernel<T, LN, false>), grid, dim3(256), 0, s, p);
 }
 
 }  // namespace
