@@ -9,20 +9,20 @@
 // Behind lengths[b] a step has delta = 0: a = 1, nothing comes in, the state passes through unchanged and every gradient is zero;
 // nothing is read there.
 //
-// Bound: N exponentials per channel and step (quarter rate) and four (forward) to twelve (backward) plain operations each; the
-// bytes of u, dt, z and out come close to that for N = 16.  So the recurrence is laid out for the vector unit: a lane owns 4 states
-// of one channel, LN = N / 4 lanes a channel, and a sum over the states is log2(LN) lane permutations inside an operand.  A
-// workgroup of up to four waves takes CH = min(64, 256 / LN) channels and goes through time in tiles of 16 steps, staged in LDS: the
-// softplus and the gate are computed once per channel and step, where the tile is loaded, in 16-byte pieces along the channels; the
-// loads of the next tile are in flight during the recurrence of this one.
+// Bound: the vector unit.  A state and step costs one exponential (10.5 cycles of its SIMD for a wave, 3.2 for a plain operation) and
+// three (forward) to twelve (backward) plain operations; the bytes of u, dt, z and out come second for N = 16.  A lane owns 4 states
+// of one channel, N / 4 lanes a channel: four independent chains and one exchange of the sum over the states, in LDS.  Time goes by in
+// tiles of 16 steps, between two kinds of waves (below).  8 sequences of 2048 steps and channels, N = 16, bfloat16, counters of the
+// vector unit busy 80 % (forward, 180 us, 1.9 TB/s) and 82 % (backward, 480 us); one kind of waves that staged, ran and wrote in turn
+// took 316 and 770 us.
 //
-// Time is cut into chunks only where batch and channels do not fill the chip (chunk_count): then a first launch runs every chunk from a
+// Time is cut into chunks only where batch and channels do not fill the chip (chunks_of): then a first launch runs every chunk from a
 // zero state, a second one joins the chunk ends (h_end = exp(A sum delta) h_start + h_local), and the main launch starts from those.
 //
 // Training: the forward pass keeps the state at the start of every tile, so the backward pass redoes 16 steps at a time in registers
-// (64 decays and 64 states per lane) and goes back over them.  dB and dC are sums over the channels: over a wave by lane exchanges
-// that halve the number of values at each level, over the workgroup's waves in LDS, over the workgroups through partials and a last
-// launch.  All sums have a fixed order; there are no atomics.
+// (64 decays and 64 states per lane) and goes back over them.  dB and dC are sums over the channels: over a wave's channels by lane
+// exchanges, over the workgroup's waves in LDS, over the workgroups through partials and a last launch.  All sums have a fixed order;
+// there are no atomics.
 #include "avsi_common.h"
 #include "avsi_wave.h"
 
@@ -944,12 +944,15 @@ int lanes_of(const avsi_scan_args* a) { return padded(a) / 4; }
 int step_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 int block_channels(int LN) { return LN <= 4 ? 64 : 256 / LN; }
 
-// Chunks of time: none where the batch and the channels leave a wave for each of the 1024 SIMDs -- the first launch over the chunks
-// costs three quarters of the main one --, else as many as make two, of at least 64 steps.
+// Chunks of time, of at least 64 steps: as many as give two workgroups to each CU (2048 waves of consumers) and not one more, so that
+// no CU gets a third; none where batch and channels leave one for three of four CUs -- the launch over the chunks costs two thirds of
+// the main one.  2048 steps, N = 16, forward / backward in us, uncut against cut: 2 sequences of 2048 channels (64 workgroups) 159 / 455
+// against 72 / 167 in 8 chunks (92 / 217 in 6, 85 / 199 in 10); 4 (128) 160 / 463 against 130 / 309 in 4; 6 (192) 163 / 466 against
+// 199 / 538 in 2, 183 / 452 in 4.
 void chunks_of(const avsi_scan_args* a, int* chunk, int* chunks) {
     const int LN = lanes_of(a), CH = block_channels(LN);
     const int64_t waves = (int64_t)a->batch * a->groups * avsi_ceil_div(a->dim / a->groups, CH) * (CH * LN / 64);
-    int64_t n = waves >= 1024 ? 1 : avsi_ceil_div(2048, waves);
+    int64_t n = waves >= 768 ? 1 : 2048 / waves;
     const int64_t most = avsi_ceil_div(a->time, 64);
     n = n < most ? n : most;
     *chunk = (int)avsi_round_up(avsi_ceil_div(a->time, n), TT);
