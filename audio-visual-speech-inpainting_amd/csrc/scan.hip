@@ -964,8 +964,9 @@ bool shape_ok(const avsi_scan_args* a) {
            a->groups > 0 && a->dim % a->groups == 0;
 }
 
-// A tile's rows are addressed with 32 bits from its first one.
+// A tile's rows are addressed with 32 bits from its first one.  (A single step has no second row: any stride will do.)
 bool strides_ok(const avsi_scan_args* a) {
+    if (a->time == 1) return true;
     const int64_t most = (int64_t)1 << 26;
     for (int64_t s : {a->u_stride[1], a->dt_stride[1], a->z_stride[1], a->dout_stride[1], a->out_stride[1], a->B_stride[1], a->C_stride[1]})
         if (s < 0 || s > most) return false;
