@@ -42,7 +42,7 @@ struct top_bits {
 };
 
 // Four codes of x * inv, the block's scale.  `top`: the block's largest absolute value.
-__device__ __forceinline__ float block_inv(float top) { return top != 0.f ? fminf(448.f / top, 3.402823466e38f) : 0.f; }
+__device__ __forceinline__ float block_inv(float top) { return top != 0.f ? fminf(1.f / top * 448.f, 3.402823466e38f) : 0.f; }
 __device__ __forceinline__ unsigned pack4(const float (&y)[4]) {
     int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], p, true);
@@ -64,7 +64,10 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int n, unsigned c) {
         for (int i = 0; i < n; ++i) p[i] = (uint8_t)(c >> (8 * i));
 }
 
-// a += b * c and the like are written out: one rounding each, as in the formula
+// The moments, their scales and codes take one rounding per operation, in the order in which they stand here: a code next to a border
+// goes to the same side as in any other evaluation of the formula in elementary fp32 operations.  (A fused one would differ in one code
+// of some millions, by up to a sixteenth of its value, and where such a code is its block's largest in a later step the whole block
+// follows.)  The weights, which no border hangs on, take fused operations.
 template <int BITS> __global__ __launch_bounds__(256) void adamw_kernel(Table tab, Hyper h) {
     for (int i = 0; i < h.n_skip; ++i)
         if (!(h.skip[i] == 0.f)) return;
@@ -120,9 +123,10 @@ template <int BITS> __global__ __launch_bounds__(256) void adamw_kernel(Table ta
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+#pragma clang fp contract(off)
             const float gj = g[k][j] * h.scale;
-            m[k][j] = fmaf(h.b1, m[k][j], h.ob1 * gj);
-            v[k][j] = fmaf(h.b2, v[k][j], h.ob2 * gj * gj);
+            m[k][j] = h.b1 * m[k][j] + h.ob1 * gj;
+            v[k][j] = h.b2 * v[k][j] + h.ob2 * gj * gj;
             r[j] = sqrtf(v[k][j]);
             const float d = fmaf(r[j], h.root_c2, h.eps);
             w[k][j] = fmaf(-h.lr, fmaf(t.weight_decay, w[k][j], (m[k][j] * h.c1) / d), w[k][j]);
