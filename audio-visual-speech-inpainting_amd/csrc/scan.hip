@@ -26,6 +26,8 @@
 #include "avsi_common.h"
 #include "avsi_wave.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int TT = 16;          // steps per tile
@@ -53,24 +55,21 @@ __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int T) {
 }
 
 // ------------------------------------------------------------------------------------------------- what the kernels share
-// A workgroup is two halves of NT threads.  The consumers own the states: a lane NS states of a channel, LN lanes a channel.  The
-// producers stage the tile behind the one the consumers are at (softplus, gates, conversion, once per channel and step) into the
-// other half of the buffers and finish the tile in front of it (sums over the lanes of a channel, outputs): a recurrence alone is a
-// chain of dependent operations that one wave per SIMD cannot fill, and the two kinds of waves fill each other's gaps.  One barrier
-// per tile; loads are a tile ahead of their use.
+// A workgroup is two kinds of waves.  The consumers own the states: a lane NS states of a channel, LN lanes a channel.  The producers
+// stage the tile behind the one the consumers are at (softplus, gates, conversion, once per channel and step) into the other half of
+// the buffers and finish the tile in front of it (sums over the lanes of a channel, outputs): a recurrence alone is a chain of
+// dependent operations that one wave per SIMD cannot fill, and the waves fill each other's gaps.  One barrier per tile; loads are a
+// tile ahead of their use.
 template <int LN_, int NS_, bool EL = false> struct Shape {
     static constexpr int LN = LN_, NS = NS_;
     static constexpr bool ELEMENTS = EL;                    // load one by one: fewer than four channels, or states in no whole quads
     static constexpr int NP = LN * NS;                      // states with their padding
     static constexpr int CH = LN <= 4 ? 64 : 256 / LN;      // channels of a workgroup
-    static constexpr int NT = CH * LN;                      // threads of either half
-    static constexpr int NW = NT / 64;
-    static constexpr int PL = LN > 8 ? 4 : LN;              // parts in which a sum over a channel's lanes is handed to the producers
-    static constexpr int QR = CH / 4;                       // quads of channels per step
-    static constexpr int ROWS = NT / QR < TT ? NT / QR : TT;
-    static constexpr int PASSES = TT / ROWS;                // of the producers over a tile's [TT][CH]
+    static constexpr int NC = CH * LN, NW = NC / 64;        // consumers: threads, waves
+    static constexpr int QR = CH / 4, PT = QR * TT;         // quads of channels per step; producers: one per quad of a tile
+    static constexpr int PL = LN > 4 ? 4 : LN;              // parts in which a sum over a channel's lanes is handed to the producers
     static constexpr int QB = NP / 4;                       // quads of states per step
-    static constexpr int BPASSES = (TT * QB + NT - 1) / NT;  // over a tile's [TT][NP] of B and C
+    static constexpr int BPASSES = (TT * QB + PT - 1) / PT;  // of the producers over a tile's [TT][NP] of B and C
     typedef __attribute__((ext_vector_type(NS_))) float Vec;   // the states of a lane
 };
 
@@ -96,7 +95,7 @@ template <typename S> struct Place {
     }
 };
 
-// A producer's part of a tile: quad q of the channels, rows i * ROWS + row.
+// A producer's part of a tile: quad q of the channels in step `row`.
 // Nothing that loads may branch by lane (the join behind such a branch waits for the load): rows from `live` on read the last row, a
 // quad that goes over the last of all channels takes the last four and is shifted when it is used; what a group does not own is
 // masked where it is used.
@@ -111,30 +110,32 @@ template <typename S> struct Stage {
 #pragma unroll
         for (int k = 0; k < 4; ++k) on[k] = 4 * q + k < at.n;
     }
-    __device__ __forceinline__ bool stages() const { return 4 * S::LN <= TT || row < S::ROWS; }       // (wide states: some threads have no row)
 };
-// Row `i`'s place inside a tile that has `rows` rows left: 32 bits, on top of the tile's uniform address.
-__device__ __forceinline__ unsigned row_at(int i, int rows, int ts) { return (unsigned)((i < rows ? i : rows - 1) * ts); }
+// Row `i`'s place inside a tile that has `rows` rows left: bytes in 32 bits, on top of the tile's uniform address.
+template <typename T> __device__ __forceinline__ unsigned row_at(int i, int rows, int64_t ts) {
+    const unsigned step = (unsigned)ts * sizeof(T), at = i * step, last = ((rows < TT ? rows : TT) - 1) * step;
+    return at < last ? at : last;
+}
+template <typename T> __device__ __forceinline__ T* at_byte(T* p, unsigned offset) {
+    return (T*)((typename std::conditional<std::is_const<T>::value, const char, char>::type*)p + offset);
+}
 
 template <typename T, typename S> struct Tile {
-    avsi_quad<T> v[S::PASSES];
+    avsi_quad<T> v;
     __device__ __forceinline__ void load(const void* base, int64_t bs, int64_t ts, const Scan& p, const Place<S>& at, const Stage<S>& st, int t0) {
         const T* b = (const T*)base + at.b * bs + t0 * ts;
+        const unsigned r = row_at<T>(st.row, at.live - t0, ts);
+        if (!S::ELEMENTS) {
+            v.load(at_byte(b, r + st.c * (unsigned)sizeof(T)));
+        } else {
+            float f[4];
 #pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            const unsigned r = row_at(i * S::ROWS + st.row, at.live - t0, (int)ts);
-            if (!S::ELEMENTS) {
-                v[i].load(b + (r + st.c));
-            } else {
-                float f[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) f[k] = (float)b[r + (st.c + k < p.dim ? st.c + k : p.dim - 1)];
-                v[i].set(f);
-            }
+            for (int k = 0; k < 4; ++k) f[k] = (float)*at_byte(b, r + (st.c + k < p.dim ? st.c + k : p.dim - 1) * (unsigned)sizeof(T));
+            v.set(f);
         }
     }
-    __device__ __forceinline__ void get(int i, const Place<S>& at, const Stage<S>& st, float (&f)[4]) const {
-        v[i].get(f);
+    __device__ __forceinline__ void get(const Place<S>& at, const Stage<S>& st, float (&f)[4]) const {
+        v.get(f);
         if (!S::ELEMENTS && at.ragged) {            // (a branch of the whole launch)
             const int shift = at.d0 + 4 * st.q - st.c;
             if (shift & 1) f[0] = f[1], f[1] = f[2], f[2] = f[3];
@@ -149,14 +150,14 @@ template <typename T, typename S> struct TileBC {
         const T* b = (const T*)base + at.b * bs + at.g * gs + t0 * ts;
 #pragma unroll
         for (int i = 0; i < S::BPASSES; ++i) {
-            const int id = i * S::NT + st.id, n = 4 * (id % S::QB);
-            const unsigned r = row_at(id / S::QB % TT, at.live - t0, (int)ts);
+            const int id = i * S::PT + st.id, n = 4 * (id % S::QB);
+            const unsigned r = row_at<T>(id / S::QB % TT, at.live - t0, ts);
             if (!S::ELEMENTS) {
-                v[i].load(b + (r + (n < p.N ? n : p.N - 4)));
+                v[i].load(at_byte(b, r + (n < p.N ? n : p.N - 4) * (unsigned)sizeof(T)));
             } else {
                 float f[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) f[k] = (float)b[r + (n + k < p.N ? n + k : p.N - 1)];
+                for (int k = 0; k < 4; ++k) f[k] = (float)*at_byte(b, r + (n + k < p.N ? n + k : p.N - 1) * (unsigned)sizeof(T));
                 v[i].set(f);
             }
         }
@@ -164,12 +165,12 @@ template <typename T, typename S> struct TileBC {
     __device__ __forceinline__ void put(avsi_f4* lds, const Scan& p, const Place<S>& at, const Stage<S>& st, int t0) const {   // [TT][NP]
 #pragma unroll
         for (int i = 0; i < S::BPASSES; ++i) {
-            const int id = i * S::NT + st.id, n = 4 * (id % S::QB);
+            const int id = i * S::PT + st.id, n = 4 * (id % S::QB);
             float f[4];
             v[i].get(f);
 #pragma unroll
             for (int k = 0; k < 4; ++k) f[k] = n + k < p.N && t0 + id / S::QB < at.live ? f[k] : 0.f;
-            if (S::BPASSES * S::NT == TT * S::QB || id < TT * S::QB) lds[id] = avsi_f4{f[0], f[1], f[2], f[3]};
+            if (S::BPASSES * S::PT == TT * S::QB || id < TT * S::QB) lds[id] = avsi_f4{f[0], f[1], f[2], f[3]};
         }
     }
 };
@@ -222,14 +223,20 @@ template <typename S> __device__ __forceinline__ void lane_start(const Scan& p, 
     }
 }
 
-// A sum over a channel's lanes: one value per lane into LDS, [channel][PL], and four channels' sums out of it.  Sixteen lanes hand
-// over four values (the buffers would not fit otherwise), the lanes that hold the same one all write it.
+// A sum over a channel's lanes: one value per lane into LDS, [channel][PL], and four channels' sums out of it.  More than four lanes
+// hand over four values (the buffers would not fit otherwise); the lanes that then hold the same one all write it.
 template <typename S> __device__ __forceinline__ void put_part(avsi_f4* row, float v) {
+    int part = threadIdx.x % S::LN;
+    if (S::LN == 8) {
+        v += avsi_dpp<0x141>(v);            // row_half_mirror
+        part = part < 4 ? part : 7 - part;
+    }
     if (S::LN == 16) {
         v += avsi_dpp<0x128>(v);            // row_ror 8
         v += avsi_dpp<0x124>(v);            // row_ror 4
+        part &= 3;
     }
-    ((float*)row)[threadIdx.x / S::LN * S::PL + threadIdx.x % S::PL] = v;
+    ((float*)row)[threadIdx.x / S::LN * S::PL + part] = v;
 }
 template <typename S> __device__ __forceinline__ void lane_sums(const avsi_f4* row, int q, float (&f)[4]) {
     constexpr int PL = S::PL, V = PL < 4 ? PL : 4;
@@ -252,13 +259,13 @@ __host__ __device__ __forceinline__ int64_t partial_stride(int dim, int NP) { re
 // ------------------------------------------------------------------------------------------------------------- forward
 // The consumers' decays are a group of two steps ahead of the states, and the operands of a group are read from LDS during the one
 // before; the fences keep the compiler from moving the reads back to their use.
-template <typename T, typename S> __global__ __launch_bounds__(2 * S::NT) void scan_fwd_kernel(Scan p) {
+template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) void scan_fwd_kernel(Scan p) {
     typedef typename S::Vec Vec;
     __shared__ avsi_f2 s_in[2][TT][S::CH];             // delta, delta u
     __shared__ avsi_f4 s_B[2][TT * S::QB], s_C[2][TT * S::QB];
     __shared__ avsi_f4 s_y[2][TT][S::CH * S::PL / 4];          // C . h of each lane's states
     const Place<S> at(p, blockIdx.y);
-    if (threadIdx.x < S::NT) {
+    if (threadIdx.x < S::NC) {
         const int ch = threadIdx.x / S::LN, ql = threadIdx.x % S::LN;
         float A[S::NS], h[S::NS];
         lane_A<S>(p, at, A);
@@ -321,100 +328,111 @@ template <typename T, typename S> __global__ __launch_bounds__(2 * S::NT) void s
                 if (S::NS * ql + j < p.N) p.state_out[((int64_t)at.b * p.dim + at.d0 + ch) * p.N + S::NS * ql + j] = h[j];
         return;
     }
-    const Stage<S> st(p, at, threadIdx.x - S::NT);
+    const Stage<S> st(p, at, threadIdx.x - S::NC);
     float bias[4], Dq[4];
     quad_of<S>(p.bias, at, st, bias);
     quad_of<S>(p.D, at, st, Dq);
-    T* out = (T*)p.out + at.b * p.ob + at.d0 + 4 * st.q;
-    Tile<T, S> u, dt, z;
-    TileBC<T, S> Bt, Ct;
+    T* out = (T*)p.out + at.b * p.ob + at.d0;
+    const unsigned place = (st.row * (unsigned)p.ot + 4 * st.q) * (unsigned)sizeof(T);          // in a tile
+    struct Ahead {              // a tile's operands in flight, two tiles ahead of their use
+        Tile<T, S> u, dt, z;
+        TileBC<T, S> B, C;
+    } x;
     auto load = [&](int n) {
         const int t0 = at.begin + (n < at.tiles ? n : at.tiles - 1) * TT;
-        u.load(p.u, p.ub, p.ut, p, at, st, t0);
-        dt.load(p.dt, p.tb, p.tt, p, at, st, t0);
-        z.load(p.z, p.zb, p.zt, p, at, st, t0);
-        Bt.load(p.B, p.Bb, p.Bt, p.Bg, p, at, st, t0);
-        Ct.load(p.C, p.Cb, p.Ct, p.Cg, p, at, st, t0);
+        x.u.load(p.u, p.ub, p.ut, p, at, st, t0);
+        x.dt.load(p.dt, p.tb, p.tt, p, at, st, t0);
+        x.z.load(p.z, p.zb, p.zt, p, at, st, t0);
+        x.B.load(p.B, p.Bb, p.Bt, p.Bg, p, at, st, t0);
+        x.C.load(p.C, p.Cb, p.Ct, p.Cg, p, at, st, t0);
     };
-    float thru[3][S::PASSES][4], gate[3][S::PASSES][4];         // D u and the gate, of the tiles n - 1, n and n + 1
-    auto stage = [&](int n) {
+    struct Held {                // D u and the gate of a tile
+        float thru[4], gate[4];
+    } even, odd;
+    float uf[4], df[4], zf[4];
+    auto take = [&](int n) {
         const int t0 = at.begin + n * TT, buf = n & 1;
-        float uf[S::PASSES][4], df[S::PASSES][4], zf[S::PASSES][4];
-#pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            u.get(i, at, st, uf[i]);
-            dt.get(i, at, st, df[i]);
-            z.get(i, at, st, zf[i]);
-        }
-        Bt.put(s_B[buf], p, at, st, t0);
-        Ct.put(s_C[buf], p, at, st, t0);
+        x.u.get(at, st, uf);
+        x.dt.get(at, st, df);
+        x.z.get(at, st, zf);
+        x.B.put(s_B[buf], p, at, st, t0);
+        x.C.put(s_C[buf], p, at, st, t0);
         load(n + 1);
+    };
+    auto stage = [&](int n, Held& w) {
+        const int t0 = at.begin + n * TT, buf = n & 1;
+        float d[4];
 #pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            float d[4];
+        for (int k = 0; k < 4; ++k) {
+            const bool on = st.on[k] && t0 + st.row < at.live;
+            const float s = step_size(df[k] + bias[k], p.softplus), g = zf[k] * avsi_sigmoid(zf[k]);
+            d[k] = on ? s : 0.f;
+            uf[k] = on ? uf[k] : 0.f;
+            w.thru[k] = Dq[k] * uf[k];
+            w.gate[k] = p.gated ? g : 1.f;
+        }
+        avsi_f4* to = (avsi_f4*)&s_in[buf][st.row][4 * st.q];
+        to[0] = avsi_f4{d[0], d[0] * uf[0], d[1], d[1] * uf[1]};
+        to[1] = avsi_f4{d[2], d[2] * uf[2], d[3], d[3] * uf[3]};
+    };
+    auto write = [&](int n, const Held& w) {
+        const int t = at.begin + n * TT + st.row;
+        if (t < at.end) {
+            float o[4];
+            lane_sums<S>(s_y[n & 1][st.row], st.q, o);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool on = st.on[k] && t0 + i * S::ROWS + st.row < at.live;
-                const float s = step_size(df[i][k] + bias[k], p.softplus), g = zf[i][k] * avsi_sigmoid(zf[i][k]);
-                d[k] = on ? s : 0.f;
-                uf[i][k] = on ? uf[i][k] : 0.f;
-                thru[2][i][k] = Dq[k] * uf[i][k];
-                gate[2][i][k] = p.gated ? g : 1.f;
-            }
-            if (st.stages()) {
-                avsi_f4* to = (avsi_f4*)&s_in[buf][i * S::ROWS + st.row][4 * st.q];
-                to[0] = avsi_f4{d[0], d[0] * uf[i][0], d[1], d[1] * uf[i][1]};
-                to[1] = avsi_f4{d[2], d[2] * uf[i][2], d[3], d[3] * uf[i][3]};
-            }
+            for (int k = 0; k < 4; ++k) o[k] = t < at.live ? (o[k] + w.thru[k]) * w.gate[k] : 0.f;
+            put_quad<T>(at_byte(out + (at.begin + n * TT) * p.ot, place), at.n - 4 * st.q, o);
         }
     };
-    auto write = [&](int n) {
-#pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            const int r = i * S::ROWS + st.row, t = at.begin + n * TT + r;
-            if (st.stages() && t < at.end) {
-                float o[4];
-                lane_sums<S>(s_y[n & 1][r], st.q, o);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) o[k] = t < at.live ? (o[k] + thru[0][i][k]) * gate[0][i][k] : 0.f;
-                put_quad<T>(out + (int64_t)t * p.ot, at.n - 4 * st.q, o);
-            }
-        }
-    };
-    auto turn = [&]() {
-#pragma unroll
-        for (int i = 0; i < S::PASSES; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                thru[0][i][k] = thru[1][i][k], thru[1][i][k] = thru[2][i][k];
-                gate[0][i][k] = gate[1][i][k], gate[1][i][k] = gate[2][i][k];
-            }
+    // While the consumers are at tile n: tile n + 1 is staged, n - 1 finished (`w`: what is held of n - 1, then of n + 1).  The loads and
+    // then the stores are issued in front of the arithmetic, and no branch lies between a load and its use: a wait behind one is for all
+    // that is in flight.
+    auto turn = [&](int n, Held& w) {
+        take(n + 1);
+        write(n - 1, w);
+        stage(n + 1, w);
+        AVSI_LDS_BARRIER();
     };
     if (at.tiles) {
         load(0);
-        stage(0);
-        turn();
+        take(0);
+        stage(0, even);
     }
     AVSI_LDS_BARRIER();
-    for (int n = 0; n < at.tiles; ++n) {
-        if (n + 1 < at.tiles) stage(n + 1);
-        if (n > 0) write(n - 1);
-        turn();
+    if (at.tiles > 1) {
+        take(1);
+        stage(1, odd);
         AVSI_LDS_BARRIER();
+        for (int n = 1; n + 1 < at.tiles; n += 2) {
+            turn(n, even);
+            if (n + 2 >= at.tiles) break;
+            turn(n + 1, odd);
+        }
+        Held before, last;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            before.thru[k] = at.tiles % 2 ? odd.thru[k] : even.thru[k], last.thru[k] = at.tiles % 2 ? even.thru[k] : odd.thru[k];
+            before.gate[k] = at.tiles % 2 ? odd.gate[k] : even.gate[k], last.gate[k] = at.tiles % 2 ? even.gate[k] : odd.gate[k];
+        }
+        write(at.tiles - 2, before);
+        AVSI_LDS_BARRIER();
+        write(at.tiles - 1, last);
+    } else if (at.tiles) {
+        AVSI_LDS_BARRIER();
+        write(0, even);
     }
-    if (at.tiles) write(at.tiles - 1);
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    if (st.stages())
-        for (int t = at.begin + at.tiles * TT + st.row; t < at.end; t += S::ROWS) put_quad<T>(out + (int64_t)t * p.ot, at.n - 4 * st.q, zero);
+    for (int t0 = at.begin + at.tiles * TT; t0 + st.row < at.end; t0 += TT) put_quad<T>(at_byte(out + t0 * p.ot, place), at.n - 4 * st.q, zero);
 }
 
 // A chunk from a zero state: its end state and the sum of its step sizes.  BACK: the adjoint state, from behind.
-template <typename T, typename S, bool BACK> __global__ __launch_bounds__(2 * S::NT) void scan_chunk_kernel(Scan p) {
+template <typename T, typename S, bool BACK> __global__ __launch_bounds__(S::NC + S::PT) void scan_chunk_kernel(Scan p) {
     typedef typename S::Vec Vec;
     __shared__ avsi_f2 s_in[2][TT][S::CH];             // delta, delta u (BACK: dy)
     __shared__ avsi_f4 s_B[2][TT * S::QB];             // (BACK: C)
     const Place<S> at(p, blockIdx.y + (BACK ? 1 : 0));  // (the first chunk's is not needed; forward: the last one's)
-    if (threadIdx.x < S::NT) {
+    if (threadIdx.x < S::NC) {
         const int ch = threadIdx.x / S::LN, ql = threadIdx.x % S::LN;
         float A[S::NS], h[S::NS] = {}, sum = 0.f;
         lane_A<S>(p, at, A);
@@ -472,7 +490,7 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(2 * S:
         }
         return;
     }
-    const Stage<S> st(p, at, threadIdx.x - S::NT);
+    const Stage<S> st(p, at, threadIdx.x - S::NC);
     float bias[4];
     quad_of<S>(p.bias, at, st, bias);
     Tile<T, S> u, dt, z;                               // BACK: u is dout
@@ -492,36 +510,27 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(2 * S:
     };
     auto stage = [&](int n) {
         const int t0 = tile_at(n), buf = n & 1;
-        float x[S::PASSES][4], df[S::PASSES][4], zf[S::PASSES][4];
-#pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            u.get(i, at, st, x[i]);
-            dt.get(i, at, st, df[i]);
-            if (BACK) z.get(i, at, st, zf[i]);
-        }
+        float x[4], df[4], zf[4], d[4];
+        u.get(at, st, x);
+        dt.get(at, st, df);
+        if (BACK) z.get(at, st, zf);
         Bt.put(s_B[buf], p, at, st, t0);
         load(n + 1);
 #pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            float d[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool on = st.on[k] && t0 + i * S::ROWS + st.row < at.live;
-                const float s = step_size(df[i][k] + bias[k], p.softplus);
-                d[k] = on ? s : 0.f;
-                if (BACK) {
-                    const float gate = zf[i][k] * avsi_sigmoid(zf[i][k]);
-                    x[i][k] = on ? x[i][k] * (p.gated ? gate : 1.f) : 0.f;
-                } else {
-                    x[i][k] = on ? x[i][k] * s : 0.f;
-                }
-            }
-            if (st.stages()) {
-                avsi_f4* to = (avsi_f4*)&s_in[buf][i * S::ROWS + st.row][4 * st.q];
-                to[0] = avsi_f4{d[0], x[i][0], d[1], x[i][1]};
-                to[1] = avsi_f4{d[2], x[i][2], d[3], x[i][3]};
+        for (int k = 0; k < 4; ++k) {
+            const bool on = st.on[k] && t0 + st.row < at.live;
+            const float s = step_size(df[k] + bias[k], p.softplus);
+            d[k] = on ? s : 0.f;
+            if (BACK) {
+                const float gate = zf[k] * avsi_sigmoid(zf[k]);
+                x[k] = on ? x[k] * (p.gated ? gate : 1.f) : 0.f;
+            } else {
+                x[k] = on ? x[k] * s : 0.f;
             }
         }
+        avsi_f4* to = (avsi_f4*)&s_in[buf][st.row][4 * st.q];
+        to[0] = avsi_f4{d[0], x[0], d[1], x[1]};
+        to[1] = avsi_f4{d[2], x[2], d[3], x[3]};
     };
     if (at.tiles) {
         load(0);
@@ -597,16 +606,16 @@ template <typename S> __device__ __forceinline__ void channel_sums(float (&b)[S:
 
 // A tile is 16 steps forward from its kept state, decays and states staying in the registers of the consumers, and 16 steps back
 // over them.
-template <typename T, typename S> __global__ __launch_bounds__(2 * S::NT) void scan_bwd_kernel(Scan p) {
+template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) void scan_bwd_kernel(Scan p) {
     typedef typename S::Vec Vec;
     __shared__ avsi_f4 s_in[2][TT][S::CH];             // delta, delta u, dy
     __shared__ avsi_f4 s_B[2][TT * S::QB], s_C[2][TT * S::QB];
     __shared__ avsi_f4 s_y[2][TT][S::CH * S::PL / 4], s_gB[2][TT][S::CH * S::PL / 4], s_gA[2][TT][S::CH * S::PL / 4];      // sums over each lane's states
-    __shared__ float s_bc[2][S::NW][TT][2 * S::NP];
+    __shared__ alignas(16) float s_bc[2][S::NW][TT][2 * S::NP];
     const Place<S> at(p, blockIdx.y);
     auto tile_at = [&](int n) { return at.begin + (at.tiles - 1 - n) * TT; };
     float* pw = p.part_w + ((int64_t)at.b * p.chunks + at.c) * partial_stride(p.dim, S::NP);
-    if (threadIdx.x < S::NT) {
+    if (threadIdx.x < S::NC) {
         const int ch = threadIdx.x / S::LN, ql = threadIdx.x % S::LN;
         float A[S::NS], Al[S::NS], g[S::NS] = {}, dA[S::NS] = {};
         lane_A<S>(p, at, A);
@@ -700,128 +709,145 @@ template <typename T, typename S> __global__ __launch_bounds__(2 * S::NT) void s
         AVSI_LDS_BARRIER();
         return;
     }
-    const Stage<S> st(p, at, threadIdx.x - S::NT);
+    const Stage<S> st(p, at, threadIdx.x - S::NC);
     float bias[4], Dq[4], dD[4] = {}, dbias[4] = {};
     quad_of<S>(p.bias, at, st, bias);
     quad_of<S>(p.D, at, st, Dq);
-    const int64_t flat = (int64_t)at.b * p.T * p.dim + at.d0 + 4 * st.q;
+    const int64_t flat = (int64_t)at.b * p.T * p.dim + at.d0;
+    const unsigned place = (st.row * (unsigned)p.dim + 4 * st.q) * (unsigned)sizeof(T);         // in a tile
     const int left = at.n - 4 * st.q;
-    auto put = [&](int t, const float (&du)[4], const float (&ddt)[4], const float (&dz)[4]) {
-        const int64_t i = flat + (int64_t)t * p.dim;
-        put_quad<T>((T*)p.du + i, left, du);
-        put_quad<T>((T*)p.ddt + i, left, ddt);
-        if (p.gated) put_quad<T>((T*)p.dz + i, left, dz);
+    auto put = [&](int t0, const float (&du)[4], const float (&ddt)[4], const float (&dz)[4]) {
+        const int64_t i = flat + (int64_t)t0 * p.dim;
+        put_quad<T>(at_byte((T*)p.du + i, place), left, du);
+        put_quad<T>(at_byte((T*)p.ddt + i, place), left, ddt);
+        if (p.gated) put_quad<T>(at_byte((T*)p.dz + i, place), left, dz);
     };
-    Tile<T, S> u, dt, z, go;
-    TileBC<T, S> Bt, Ct;
+    struct Ahead {
+        Tile<T, S> u, dt, z, go;
+        TileBC<T, S> B, C;
+    } x;
     auto load = [&](int n) {
         const int t0 = tile_at(n < at.tiles ? n : at.tiles - 1);
-        u.load(p.u, p.ub, p.ut, p, at, st, t0);
-        dt.load(p.dt, p.tb, p.tt, p, at, st, t0);
-        go.load(p.dout, p.gb, p.gt, p, at, st, t0);
-        z.load(p.z, p.zb, p.zt, p, at, st, t0);
-        Bt.load(p.B, p.Bb, p.Bt, p.Bg, p, at, st, t0);
-        Ct.load(p.C, p.Cb, p.Ct, p.Cg, p, at, st, t0);
+        x.u.load(p.u, p.ub, p.ut, p, at, st, t0);
+        x.dt.load(p.dt, p.tb, p.tt, p, at, st, t0);
+        x.go.load(p.dout, p.gb, p.gt, p, at, st, t0);
+        x.z.load(p.z, p.zb, p.zt, p, at, st, t0);
+        x.B.load(p.B, p.Bb, p.Bt, p.Bg, p, at, st, t0);
+        x.C.load(p.C, p.Cb, p.Ct, p.Cg, p, at, st, t0);
     };
     struct Held {                // what a tile's gradients need besides the consumers' sums
         float u[4], delta[4], slope[4], dy[4], gz[4];
-    } held[3][S::PASSES];        // of the tiles n - 1, n and n + 1
-    auto stage = [&](int n) {
+    } even, odd;
+    float uf[4], df[4], zf[4], of[4];
+    auto take = [&](int n) {
         const int t0 = tile_at(n), buf = n & 1;
-        float df[S::PASSES][4], zf[S::PASSES][4], of[S::PASSES][4];
-#pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            u.get(i, at, st, held[2][i].u);
-            dt.get(i, at, st, df[i]);
-            z.get(i, at, st, zf[i]);
-            go.get(i, at, st, of[i]);
-        }
-        Bt.put(s_B[buf], p, at, st, t0);
-        Ct.put(s_C[buf], p, at, st, t0);
+        x.u.get(at, st, uf);
+        x.dt.get(at, st, df);
+        x.z.get(at, st, zf);
+        x.go.get(at, st, of);
+        x.B.put(s_B[buf], p, at, st, t0);
+        x.C.put(s_C[buf], p, at, st, t0);
         load(n + 1);
-#pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            Held& w = held[2][i];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool on = st.on[k] && t0 + i * S::ROWS + st.row < at.live;
-                const float x = df[i][k] + bias[k], d = step_size(x, p.softplus), s = avsi_sigmoid(x), e = avsi_sigmoid(zf[i][k]);
-                w.u[k] = on ? w.u[k] : 0.f;
-                w.delta[k] = on ? d : 0.f;
-                w.slope[k] = on ? (p.softplus ? s : 1.f) : 0.f;
-                w.dy[k] = on ? of[i][k] * (p.gated ? zf[i][k] * e : 1.f) : 0.f;
-                w.gz[k] = on ? of[i][k] * (e * fmaf(zf[i][k], 1.f - e, 1.f)) : 0.f;
-            }
-            if (st.stages())
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    s_in[buf][i * S::ROWS + st.row][4 * st.q + k] = avsi_f4{w.delta[k], w.delta[k] * w.u[k], w.dy[k], 0.f};
-        }
     };
-    auto finish = [&](int n) {
+    auto stage = [&](int n, Held& w) {
         const int t0 = tile_at(n), buf = n & 1;
-        for (int i = st.id; i < TT * 2 * S::NP; i += S::NT) {
-            float s = 0.f;
 #pragma unroll
-            for (int w = 0; w < S::NW; ++w) s += s_bc[buf][w][i / (2 * S::NP)][i % (2 * S::NP)];
-            const int t = t0 + i / (2 * S::NP);
-            if (t < at.live)
-                p.part_bc[((((int64_t)at.b * p.T + t) * p.groups + at.g) * p.blocks + at.block) * 2 * S::NP + i % (2 * S::NP)] = s;
-        }
-#pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) {
-            const int r = i * S::ROWS + st.row, t = t0 + r;
-            if (st.stages() && t < at.end) {
-                const Held& w = held[0][i];
-                float du[4], ddt[4], dz[4], gB[4], gA[4], y[4];
-                lane_sums<S>(s_gB[buf][r], st.q, gB);
-                lane_sums<S>(s_gA[buf][r], st.q, gA);
-                lane_sums<S>(s_y[buf][r], st.q, y);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {           // (behind a length everything held is zero)
-                    du[k] = fmaf(Dq[k], w.dy[k], w.delta[k] * gB[k]);
-                    ddt[k] = fmaf(w.u[k], gB[k], gA[k]) * w.slope[k];
-                    dz[k] = w.gz[k] * fmaf(Dq[k], w.u[k], y[k]);
-                    dD[k] = fmaf(w.dy[k], w.u[k], dD[k]);
-                    dbias[k] += ddt[k];
-                    if (t >= at.live) du[k] = ddt[k] = dz[k] = 0.f;
-                }
-                put(t, du, ddt, dz);
-            }
+        for (int k = 0; k < 4; ++k) {
+            const bool on = st.on[k] && t0 + st.row < at.live;
+            const float x = df[k] + bias[k], d = step_size(x, p.softplus), s = avsi_sigmoid(x), e = avsi_sigmoid(zf[k]);
+            w.u[k] = on ? uf[k] : 0.f;
+            w.delta[k] = on ? d : 0.f;
+            w.slope[k] = on ? (p.softplus ? s : 1.f) : 0.f;
+            w.dy[k] = on ? of[k] * (p.gated ? zf[k] * e : 1.f) : 0.f;
+            w.gz[k] = on ? of[k] * (e * fmaf(zf[k], 1.f - e, 1.f)) : 0.f;
+            s_in[buf][st.row][4 * st.q + k] = avsi_f4{w.delta[k], w.delta[k] * w.u[k], w.dy[k], 0.f};
         }
     };
-    auto turn = [&]() {
+    auto finish = [&](int n, const Held& w) {
+        const int t0 = tile_at(n), buf = n & 1;
+        constexpr int ROW = 2 * S::NP;
 #pragma unroll
-        for (int i = 0; i < S::PASSES; ++i) held[0][i] = held[1][i], held[1][i] = held[2][i];
+        for (int i0 = 0; i0 < TT * ROW; i0 += 2 * S::PT) {
+            const int i = i0 + 2 * st.id, t = t0 + i / ROW;
+            if (TT * ROW % (2 * S::PT) && i >= TT * ROW) break;
+            avsi_f2 s = {0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < S::NW; ++k) s += *(const avsi_f2*)&s_bc[buf][k][i / ROW][i % ROW];
+            if (t < at.live)
+                *(avsi_f2*)(p.part_bc + ((((int64_t)at.b * p.T + t) * p.groups + at.g) * p.blocks + at.block) * ROW + i % ROW) = s;
+        }
+        const int t = t0 + st.row;
+        if (t < at.end) {
+            float du[4], ddt[4], dz[4], gB[4], gA[4], y[4];
+            lane_sums<S>(s_gB[buf][st.row], st.q, gB);
+            lane_sums<S>(s_gA[buf][st.row], st.q, gA);
+            lane_sums<S>(s_y[buf][st.row], st.q, y);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {           // (behind a length everything held is zero)
+                du[k] = fmaf(Dq[k], w.dy[k], w.delta[k] * gB[k]);
+                ddt[k] = fmaf(w.u[k], gB[k], gA[k]) * w.slope[k];
+                dz[k] = w.gz[k] * fmaf(Dq[k], w.u[k], y[k]);
+                dD[k] = fmaf(w.dy[k], w.u[k], dD[k]);
+                dbias[k] += ddt[k];
+                if (t >= at.live) du[k] = ddt[k] = dz[k] = 0.f;
+            }
+            put(t0, du, ddt, dz);
+        }
+    };
+    // While the consumers are at tile n: tile n + 1 is staged, n - 1 finished (`w`: what is held of n - 1, then of n + 1).  The loads and
+    // then the stores are issued in front of the arithmetic, and no branch lies between a load and its use: a wait behind one is for all
+    // that is in flight.
+    auto turn = [&](int n, Held& w) {
+        take(n + 1);
+        finish(n - 1, w);
+        stage(n + 1, w);
+        AVSI_LDS_BARRIER();
     };
     if (at.tiles) {
         load(0);
-        stage(0);
-        turn();
+        take(0);
+        stage(0, even);
     }
     AVSI_LDS_BARRIER();
-    for (int n = 0; n < at.tiles; ++n) {
-        if (n + 1 < at.tiles) stage(n + 1);
-        if (n > 0) finish(n - 1);
-        turn();
+    if (at.tiles > 1) {
+        take(1);
+        stage(1, odd);
         AVSI_LDS_BARRIER();
-    }
-    if (at.tiles) finish(at.tiles - 1);
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    if (st.stages())
-        for (int t = at.begin + at.tiles * TT + st.row; t < at.end; t += S::ROWS) put(t, zero, zero, zero);
-    // D's and the bias' gradients of this workgroup's channels, over its chunk: the rows of the producers
-    AVSI_LDS_BARRIER();
-    if (st.stages())
+        for (int n = 1; n + 1 < at.tiles; n += 2) {
+            turn(n, even);
+            if (n + 2 >= at.tiles) break;
+            turn(n + 1, odd);
+        }
+        Held before, last;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            ((float*)s_gB[0][st.row])[4 * st.q + k] = dD[k];
-            ((float*)s_gA[0][st.row])[4 * st.q + k] = dbias[k];
+            before.u[k] = at.tiles % 2 ? odd.u[k] : even.u[k], last.u[k] = at.tiles % 2 ? even.u[k] : odd.u[k];
+            before.delta[k] = at.tiles % 2 ? odd.delta[k] : even.delta[k], last.delta[k] = at.tiles % 2 ? even.delta[k] : odd.delta[k];
+            before.slope[k] = at.tiles % 2 ? odd.slope[k] : even.slope[k], last.slope[k] = at.tiles % 2 ? even.slope[k] : odd.slope[k];
+            before.dy[k] = at.tiles % 2 ? odd.dy[k] : even.dy[k], last.dy[k] = at.tiles % 2 ? even.dy[k] : odd.dy[k];
+            before.gz[k] = at.tiles % 2 ? odd.gz[k] : even.gz[k], last.gz[k] = at.tiles % 2 ? even.gz[k] : odd.gz[k];
         }
+        finish(at.tiles - 2, before);
+        AVSI_LDS_BARRIER();
+        finish(at.tiles - 1, last);
+    } else if (at.tiles) {
+        AVSI_LDS_BARRIER();
+        finish(0, even);
+    }
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int t0 = at.begin + at.tiles * TT; t0 + st.row < at.end; t0 += TT) put(t0, zero, zero, zero);
+    // D's and the bias' gradients of this workgroup's channels, over its chunk: the rows of the producers
+    AVSI_LDS_BARRIER();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        ((float*)s_gB[0][st.row])[4 * st.q + k] = dD[k];
+        ((float*)s_gA[0][st.row])[4 * st.q + k] = dbias[k];
+    }
     AVSI_LDS_BARRIER();
     if (st.id < at.n) {
         float sD = 0.f, sb = 0.f;
-        for (int r = 0; r < S::ROWS; ++r) {
+#pragma unroll
+        for (int r = 0; r < TT; ++r) {
             sD += ((const float*)s_gB[0][r])[st.id];
             sb += ((const float*)s_gA[0][r])[st.id];
         }
@@ -1001,17 +1027,17 @@ template <bool BACK> void go_join(const Scan& p, hipStream_t s) {
 }
 template <typename T, typename S> void go_fwd(const Scan& p, hipStream_t s) {
     if (p.chunks > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, S, false>), dim3(p.groups * p.blocks, p.chunks - 1, p.batch), dim3(2 * S::NT), 0, s, p);
+        hipLaunchKernelGGL((scan_chunk_kernel<T, S, false>), dim3(p.groups * p.blocks, p.chunks - 1, p.batch), dim3(S::NC + S::PT), 0, s, p);
         go_join<false>(p, s);
     }
-    hipLaunchKernelGGL((scan_fwd_kernel<T, S>), dim3(p.groups * p.blocks, p.chunks, p.batch), dim3(2 * S::NT), 0, s, p);
+    hipLaunchKernelGGL((scan_fwd_kernel<T, S>), dim3(p.groups * p.blocks, p.chunks, p.batch), dim3(S::NC + S::PT), 0, s, p);
 }
 template <typename T, typename S> void go_bwd(const Scan& p, hipStream_t s) {
     if (p.chunks > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, S, true>), dim3(p.groups * p.blocks, p.chunks - 1, p.batch), dim3(2 * S::NT), 0, s, p);
+        hipLaunchKernelGGL((scan_chunk_kernel<T, S, true>), dim3(p.groups * p.blocks, p.chunks - 1, p.batch), dim3(S::NC + S::PT), 0, s, p);
         go_join<true>(p, s);
     }
-    hipLaunchKernelGGL((scan_bwd_kernel<T, S>), dim3(p.groups * p.blocks, p.chunks, p.batch), dim3(2 * S::NT), 0, s, p);
+    hipLaunchKernelGGL((scan_bwd_kernel<T, S>), dim3(p.groups * p.blocks, p.chunks, p.batch), dim3(S::NC + S::PT), 0, s, p);
 }
 template <typename T, int LN> void go_step(const Scan& p, hipStream_t s) {
     // as many workgroups as stay on the chip (eight a CU), each over several sequences
