@@ -223,9 +223,15 @@ template <typename S> __device__ __forceinline__ void lane_start(const Scan& p, 
     }
 }
 
+// Where a channel's 16 (8) bytes lie in a row of LDS: sixteen producers in a row read or write the same channel of their quads at 64 (32)
+// bytes from each other, which is one bank in four (two); so the channels inside a quad are permuted from quad to quad.  (With them in
+// order the backward pass spent a quarter of its LDS cycles on conflicts.)
+template <typename S> __device__ __forceinline__ int place16(int row, int ch) { return ch ^ ((row * S::QR + (ch >> 2)) >> 2 & 3); }
+template <typename S> __device__ __forceinline__ int place8(int row, int ch) { return ch ^ ((row * S::QR + (ch >> 2)) >> 3 & 1) << 1; }
+
 // A sum over a channel's lanes: one value per lane into LDS, [channel][PL], and four channels' sums out of it.  More than four lanes
 // hand over four values (the buffers would not fit otherwise); the lanes that then hold the same one all write it.
-template <typename S> __device__ __forceinline__ void put_part(avsi_f4* row, float v) {
+template <typename S> __device__ __forceinline__ void put_part(avsi_f4 (*rows)[S::CH * S::PL / 4], int t, float v) {
     int part = threadIdx.x % S::LN;
     if (S::LN == 8) {
         v += avsi_dpp<0x141>(v);            // row_half_mirror
@@ -236,17 +242,18 @@ template <typename S> __device__ __forceinline__ void put_part(avsi_f4* row, flo
         v += avsi_dpp<0x124>(v);            // row_ror 4
         part &= 3;
     }
-    ((float*)row)[threadIdx.x / S::LN * S::PL + part] = v;
+    const int ch = threadIdx.x / S::LN;
+    ((float*)rows[t])[(S::PL == 4 ? place16<S>(t, ch) : ch) * S::PL + part] = v;
 }
-template <typename S> __device__ __forceinline__ void lane_sums(const avsi_f4* row, int q, float (&f)[4]) {
+template <typename S> __device__ __forceinline__ void lane_sums(const avsi_f4 (*rows)[S::CH * S::PL / 4], int t, int q, float (&f)[4]) {
     constexpr int PL = S::PL, V = PL < 4 ? PL : 4;
-    const float* p = (const float*)row + 4 * q * PL;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+        const float* p = (const float*)rows[t] + (PL == 4 ? place16<S>(t, 4 * q + k) : 4 * q + k) * PL;
         f[k] = 0.f;
 #pragma unroll
         for (int l = 0; l < PL; l += V) {
-            const avsi_raw<float, V> r = *(const avsi_raw<float, V>*)__builtin_assume_aligned(p + k * PL + l, 4 * V);
+            const avsi_raw<float, V> r = *(const avsi_raw<float, V>*)__builtin_assume_aligned(p + l, 4 * V);
 #pragma unroll
             for (int i = 0; i < V; ++i) f[k] += r.v[i];
         }
@@ -266,6 +273,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
     __shared__ avsi_f4 s_y[2][TT][S::CH * S::PL / 4];          // C . h of each lane's states
     const Place<S> at(p, blockIdx.y);
     if (threadIdx.x < S::NC) {
+        __builtin_amdgcn_s_setprio(3);          // (they are the longer of the two: 60.4 -> 59.0 us for 8191 steps of 1536 channels)
         const int ch = threadIdx.x / S::LN, ql = threadIdx.x % S::LN;
         float A[S::NS], h[S::NS];
         lane_A<S>(p, at, A);
@@ -278,7 +286,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
             const int buf = n & 1;
             avsi_f2 in[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) in[t] = s_in[buf][t][ch];
+            for (int t = 0; t < TT; ++t) in[t] = s_in[buf][t][place8<S>(t, ch)];
             Vec Bv[2], Cv[2], Bn[2], Cn[2];
             auto fetch = [&](int t) {
 #pragma unroll
@@ -316,7 +324,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
                         h[j] = fmaf(a[k][j], h[j], in[t + k][1] * Bv[k][j]);
                         y = fmaf(h[j], Cv[k][j], y);
                     }
-                    put_part<S>(s_y[buf][t + k], y);
+                    put_part<S>(s_y[buf], t + k, y);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -371,15 +379,15 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
             w.thru[k] = Dq[k] * uf[k];
             w.gate[k] = p.gated ? g : 1.f;
         }
-        avsi_f4* to = (avsi_f4*)&s_in[buf][st.row][4 * st.q];
-        to[0] = avsi_f4{d[0], d[0] * uf[0], d[1], d[1] * uf[1]};
-        to[1] = avsi_f4{d[2], d[2] * uf[2], d[3], d[3] * uf[3]};
+        avsi_f4* to = (avsi_f4*)s_in[buf][st.row];
+        to[place8<S>(st.row, 4 * st.q) / 2] = avsi_f4{d[0], d[0] * uf[0], d[1], d[1] * uf[1]};
+        to[place8<S>(st.row, 4 * st.q + 2) / 2] = avsi_f4{d[2], d[2] * uf[2], d[3], d[3] * uf[3]};
     };
     auto write = [&](int n, const Held& w) {
         const int t = at.begin + n * TT + st.row;
         if (t < at.end) {
             float o[4];
-            lane_sums<S>(s_y[n & 1][st.row], st.q, o);
+            lane_sums<S>(s_y[n & 1], st.row, st.q, o);
 #pragma unroll
             for (int k = 0; k < 4; ++k) o[k] = t < at.live ? (o[k] + w.thru[k]) * w.gate[k] : 0.f;
             put_quad<T>(at_byte(out + (at.begin + n * TT) * p.ot, place), at.n - 4 * st.q, o);
@@ -433,6 +441,7 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(S::NC 
     __shared__ avsi_f4 s_B[2][TT * S::QB];             // (BACK: C)
     const Place<S> at(p, blockIdx.y + (BACK ? 1 : 0));  // (the first chunk's is not needed; forward: the last one's)
     if (threadIdx.x < S::NC) {
+        __builtin_amdgcn_s_setprio(3);
         const int ch = threadIdx.x / S::LN, ql = threadIdx.x % S::LN;
         float A[S::NS], h[S::NS] = {}, sum = 0.f;
         lane_A<S>(p, at, A);
@@ -443,7 +452,7 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(S::NC 
             const int buf = n & 1;
             avsi_f2 in[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) in[t] = s_in[buf][BACK ? TT - 1 - t : t][ch];
+            for (int t = 0; t < TT; ++t) in[t] = s_in[buf][BACK ? TT - 1 - t : t][place8<S>(BACK ? TT - 1 - t : t, ch)];
             Vec Bv[2], Bn[2];
             auto fetch = [&](int t) {
 #pragma unroll
@@ -528,9 +537,9 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(S::NC 
                 x[k] = on ? x[k] * s : 0.f;
             }
         }
-        avsi_f4* to = (avsi_f4*)&s_in[buf][st.row][4 * st.q];
-        to[0] = avsi_f4{d[0], x[0], d[1], x[1]};
-        to[1] = avsi_f4{d[2], x[2], d[3], x[3]};
+        avsi_f4* to = (avsi_f4*)s_in[buf][st.row];
+        to[place8<S>(st.row, 4 * st.q) / 2] = avsi_f4{d[0], x[0], d[1], x[1]};
+        to[place8<S>(st.row, 4 * st.q + 2) / 2] = avsi_f4{d[2], x[2], d[3], x[3]};
     };
     if (at.tiles) {
         load(0);
@@ -644,7 +653,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
             auto fetch = [&](int t) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    in2[j] = s_in[buf][t + j][ch];
+                    in2[j] = s_in[buf][t + j][place16<S>(t + j, ch)];
                     Bn[j] = ((const Vec*)s_B[buf])[(t + j) * S::LN + ql];
                     Cn[j] = ((const Vec*)s_C[buf])[(t + j) * S::LN + ql];
                 }
@@ -669,7 +678,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
                         h[j] = fmaf(a[t + k][j], h[j], in[k][1] * Bv[k][j]);
                         y = fmaf(h[j], Cv[k][j], y);
                     }
-                    put_part<S>(s_y[buf][t + k], y);
+                    put_part<S>(s_y[buf], t + k, y);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -694,8 +703,8 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
                         gA = fmaf(x, A[j], gA);
                         dAt[j] = fmaf(x, in[k][0], dAt[j]);
                     }
-                    put_part<S>(s_gB[buf][t], gB);
-                    put_part<S>(s_gA[buf][t], gA);
+                    put_part<S>(s_gB[buf], t, gB);
+                    put_part<S>(s_gA[buf], t, gA);
                     channel_sums<S>(vb, vc, s_bc[buf][threadIdx.x >> 6][t]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -760,7 +769,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
             w.slope[k] = on ? (p.softplus ? s : 1.f) : 0.f;
             w.dy[k] = on ? of[k] * (p.gated ? zf[k] * e : 1.f) : 0.f;
             w.gz[k] = on ? of[k] * (e * fmaf(zf[k], 1.f - e, 1.f)) : 0.f;
-            s_in[buf][st.row][4 * st.q + k] = avsi_f4{w.delta[k], w.delta[k] * w.u[k], w.dy[k], 0.f};
+            s_in[buf][st.row][place16<S>(st.row, 4 * st.q + k)] = avsi_f4{w.delta[k], w.delta[k] * w.u[k], w.dy[k], 0.f};
         }
     };
     auto finish = [&](int n, const Held& w) {
@@ -779,9 +788,9 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
         const int t = t0 + st.row;
         if (t < at.end) {
             float du[4], ddt[4], dz[4], gB[4], gA[4], y[4];
-            lane_sums<S>(s_gB[buf][st.row], st.q, gB);
-            lane_sums<S>(s_gA[buf][st.row], st.q, gA);
-            lane_sums<S>(s_y[buf][st.row], st.q, y);
+            lane_sums<S>(s_gB[buf], st.row, st.q, gB);
+            lane_sums<S>(s_gA[buf], st.row, st.q, gA);
+            lane_sums<S>(s_y[buf], st.row, st.q, y);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {           // (behind a length everything held is zero)
                 du[k] = fmaf(Dq[k], w.dy[k], w.delta[k] * gB[k]);
