@@ -10,11 +10,11 @@
 // nothing is read there.
 //
 // Bound: the vector unit.  A state and step costs one exponential (10.5 cycles of its SIMD for a wave, 3.2 for a plain operation) and
-// three (forward) to twelve (backward) plain operations; the bytes of u, dt, z and out come second for N = 16.  A lane owns 4 states
+// four (forward) to twelve (backward) plain operations; the bytes of u, dt, z and out come second for N = 16.  A lane owns 4 states
 // of one channel, N / 4 lanes a channel: four independent chains and one exchange of the sum over the states, in LDS.  Time goes by in
-// tiles of 16 steps, between two kinds of waves (below).  8 sequences of 2048 steps and channels, N = 16, bfloat16, counters of the
-// vector unit busy 80 % (forward, 180 us, 1.9 TB/s) and 82 % (backward, 480 us); one kind of waves that staged, ran and wrote in turn
-// took 316 and 770 us.
+// tiles of 16 steps, between two kinds of waves (below).  8 sequences of 2048 steps and channels, N = 16, bfloat16: forward 169 us
+// (2.4 TB/s with the states it keeps, the vector unit's counter at 81 %), backward 473 us (82 %); one kind of waves that staged, ran and
+// wrote in turn took 316 and 770 us.
 //
 // Time is cut into chunks only where batch and channels do not fill the chip (chunks_of): then a first launch runs every chunk from a
 // zero state, a second one joins the chunk ends (h_end = exp(A sum delta) h_start + h_local), and the main launch starts from those.
@@ -980,10 +980,10 @@ int step_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32
 int block_channels(int LN) { return LN <= 4 ? 64 : 256 / LN; }
 
 // Chunks of time, of at least 64 steps: as many as give two workgroups to each CU (2048 waves of consumers) and not one more, so that
-// no CU gets a third; none where batch and channels leave one for three of four CUs -- the launch over the chunks costs two thirds of
-// the main one.  2048 steps, N = 16, forward / backward in us, uncut against cut: 2 sequences of 2048 channels (64 workgroups) 159 / 455
-// against 72 / 167 in 8 chunks (92 / 217 in 6, 85 / 199 in 10); 4 (128) 160 / 463 against 130 / 309 in 4; 6 (192) 163 / 466 against
-// 199 / 538 in 2, 183 / 452 in 4.
+// no CU gets a third; none where batch and channels leave one for three of four CUs -- the launch over the chunks costs three quarters
+// of the main one.  2048 steps, N = 16, a whole forward / backward call in us: 2 sequences of 2048 channels (64 workgroups) 146 / 431
+// uncut, 67 / 158 in 8 chunks (85 / 204 in 6, 79 / 188 in 10); 4 (128) 147 / 439 uncut, 120 / 291 in 4; 6 (192) 152 / 445 uncut,
+// 185 / 514 in 2, 175 / 428 in 4.
 void chunks_of(const avsi_scan_args* a, int* chunk, int* chunks) {
     const int LN = lanes_of(a), CH = block_channels(LN);
     const int64_t waves = (int64_t)a->batch * a->groups * avsi_ceil_div(a->dim / a->groups, CH) * (CH * LN / 64);
@@ -995,8 +995,8 @@ void chunks_of(const avsi_scan_args* a, int* chunk, int* chunks) {
 }
 
 bool shape_ok(const avsi_scan_args* a) {
-    return a && avsi_dtype_ok(a->dtype) && a->batch > 0 && a->batch <= 65535 && a->time > 0 && a->dim > 0 && a->dim <= (1 << 26) && a->state > 0 &&
-           a->groups > 0 && a->dim % a->groups == 0;
+    return a && avsi_dtype_ok(a->dtype) && a->batch > 0 && a->batch <= 65535 && a->time > 0 && a->time <= (1 << 30) && a->dim > 0 &&
+           a->dim <= (1 << 26) && a->state > 0 && a->groups > 0 && a->dim % a->groups == 0;
 }
 
 // A tile's rows are addressed with 32 bits from its first one.  (A single step has no second row: any stride will do.)

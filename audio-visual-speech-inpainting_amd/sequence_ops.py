@@ -367,6 +367,10 @@ def selective_scan_step(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=T
     bsz, dim = u.shape
     N, operands = _scan_operands(what, u, dt, A, B, C, D, z, dt_bias, softplus)
     _state(what, state, (bsz, dim, N), torch.float32)
+    lo = state.data_ptr()
+    hi = lo + 4 * bsz * dim * N
+    if any(p and lo <= p < hi for p in operands[8:13]):         # (u, dt, z, B, C)
+        _bad("%s: the inputs must not be part of the state", what)
     dev = _device(what, u, dt, A, B, C, D, z, dt_bias, state)
     out = u.new_empty((bsz, dim))
     if bsz:

@@ -733,6 +733,7 @@ int avsi_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_
  *   w [dim][taps], bias [dim] (or NULL), dw, dbias: float
  *   state          `dtype` [batch][taps - 1][dim]: the inputs in front of x[0], oldest first; NULL: zeros.  It is a
  *                  constant of the backward pass
+ *   time           at most 2^30
  *   lengths        device int32 [batch] or NULL: sequence b has min(max(lengths[b], 0), time) steps; behind them y and dx
  *                  are zero and x, dy are not read
  *   state_out      `dtype` [batch][taps - 1][dim] or NULL: the last inputs in front of each sequence's end (not `state`)
@@ -757,7 +758,8 @@ int avsi_causal_conv_step(const void* x, int64_t x_stride_b, int dtype, const fl
  *   u, dt, z, dout   `dtype` [batch][time][dim], strides {batch, time}, unit stride along the channels; z may be NULL
  *   B, C             `dtype` [batch][time][groups][state], strides {batch, time, group}, unit stride along the states;
  *                    channel d belongs to group d / (dim / groups)
- *   A [dim][state], D [dim] or NULL (0), dt_bias [dim] or NULL (0): float.  state <= 64, batch <= 65535
+ *   A [dim][state], D [dim] or NULL (0), dt_bias [dim] or NULL (0): float.  state <= 64, batch <= 65535,
+ *                    time <= 2^30, dim <= 2^26; strides of time from 0 to 2^26 unless time is 1
  *   state_in         float [batch][dim][state] or NULL (zeros), a constant of the backward pass; state_out: the state at each
  *                    sequence's end, or NULL (not state_in)
  *   lengths          as for the convolution: behind its length a sequence's state stands still, out and all gradients are
@@ -769,7 +771,8 @@ int avsi_causal_conv_step(const void* x, int64_t x_stride_b, int dtype, const fl
  *                    [batch][time][groups][state] contiguous; dA [dim][state], dD [dim], ddt_bias [dim]: float (dD,
  *                    ddt_bias may be NULL)
  * States, sums and statistics are float; every sum has a fixed order.  The step takes one token per sequence (time = 1,
- * strides of time unused) and moves the states in `state_out` on in place (state_in, lengths, kept unused).
+ * strides of time unused) and moves the states in `state_out`, which share no memory with the inputs, on in place
+ * (state_in, lengths, kept unused).
  * ------------------------------------------------------------------------------------ */
 typedef struct avsi_scan_args {
     int32_t dtype, batch, time, dim, state, groups, softplus, reserved;
