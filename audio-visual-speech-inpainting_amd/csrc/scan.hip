@@ -168,8 +168,9 @@ template <typename T, typename S> struct TileBC {
             const int id = i * S::PT + st.id, n = 4 * (id % S::QB);
             float f[4];
             v[i].get(f);
+            if (t0 + TT > at.live || p.N < S::NP)       // (uniform)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) f[k] = n + k < p.N && t0 + id / S::QB < at.live ? f[k] : 0.f;
+                for (int k = 0; k < 4; ++k) f[k] = n + k < p.N && t0 + id / S::QB < at.live ? f[k] : 0.f;
             if (S::BPASSES * S::PT == TT * S::QB || id < TT * S::QB) lds[id] = avsi_f4{f[0], f[1], f[2], f[3]};
         }
     }
@@ -181,9 +182,14 @@ template <typename T> __device__ __forceinline__ void put_quad(T* p, int n, cons
 }
 
 // (both values and a choice: a branch, though one of the whole launch, would fence the schedule)
-__device__ __forceinline__ float step_size(float x, int softplus) {
-    const float s = avsi_softplus(x);
+__device__ __forceinline__ float step_size(float x, int softplus, float& slope) {
+    const float s = avsi_softplus(x, slope);
+    slope = softplus ? slope : 1.f;
     return softplus ? s : x;
+}
+__device__ __forceinline__ float step_size(float x, int softplus) {
+    float slope;
+    return step_size(x, softplus, slope);
 }
 
 // dt_bias, D of this thread's quad of channels
@@ -372,12 +378,15 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
         float d[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const bool on = st.on[k] && t0 + st.row < at.live;
-            const float s = step_size(df[k] + bias[k], p.softplus), g = zf[k] * avsi_sigmoid(zf[k]);
-            d[k] = on ? s : 0.f;
-            uf[k] = on ? uf[k] : 0.f;
+            const float g = zf[k] * avsi_sigmoid(zf[k]);
+            d[k] = step_size(df[k] + bias[k], p.softplus);
             w.thru[k] = Dq[k] * uf[k];
             w.gate[k] = p.gated ? g : 1.f;
+        }
+        if (t0 + TT > at.live) {         // (uniform; what lanes without a channel compute goes nowhere)
+            const bool on = t0 + st.row < at.live;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) d[k] = on ? d[k] : 0.f, uf[k] = on ? uf[k] : 0.f;
         }
         avsi_f4* to = (avsi_f4*)s_in[buf][st.row];
         to[place8<S>(st.row, 4 * st.q) / 2] = avsi_f4{d[0], d[0] * uf[0], d[1], d[1] * uf[1]};
@@ -389,7 +398,10 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
             float o[4];
             lane_sums<S>(s_y[n & 1], st.row, st.q, o);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = t < at.live ? (o[k] + w.thru[k]) * w.gate[k] : 0.f;
+            for (int k = 0; k < 4; ++k) o[k] = (o[k] + w.thru[k]) * w.gate[k];
+            if (at.begin + (n + 1) * TT > at.live)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = t < at.live ? o[k] : 0.f;
             put_quad<T>(at_byte(out + (at.begin + n * TT) * p.ot, place), at.n - 4 * st.q, o);
         }
     };
@@ -519,7 +531,7 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(S::NC 
     };
     auto stage = [&](int n) {
         const int t0 = tile_at(n), buf = n & 1;
-        float x[4], df[4], zf[4], d[4];
+        float x[4], df[4], zf[4] = {}, d[4];
         u.get(at, st, x);
         dt.get(at, st, df);
         if (BACK) z.get(at, st, zf);
@@ -527,15 +539,14 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(S::NC 
         load(n + 1);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const bool on = st.on[k] && t0 + st.row < at.live;
-            const float s = step_size(df[k] + bias[k], p.softplus);
-            d[k] = on ? s : 0.f;
-            if (BACK) {
-                const float gate = zf[k] * avsi_sigmoid(zf[k]);
-                x[k] = on ? x[k] * (p.gated ? gate : 1.f) : 0.f;
-            } else {
-                x[k] = on ? x[k] * s : 0.f;
-            }
+            d[k] = step_size(df[k] + bias[k], p.softplus);
+            const float gate = zf[k] * avsi_sigmoid(zf[k]);
+            x[k] *= BACK ? (p.gated ? gate : 1.f) : d[k];
+        }
+        if (t0 + TT > at.live) {
+            const bool on = t0 + st.row < at.live;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) d[k] = on ? d[k] : 0.f, x[k] = on ? x[k] : 0.f;
         }
         avsi_f4* to = (avsi_f4*)s_in[buf][st.row];
         to[place8<S>(st.row, 4 * st.q) / 2] = avsi_f4{d[0], x[0], d[1], x[1]};
@@ -762,13 +773,21 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
         const int t0 = tile_at(n), buf = n & 1;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const bool on = st.on[k] && t0 + st.row < at.live;
-            const float x = df[k] + bias[k], d = step_size(x, p.softplus), s = avsi_sigmoid(x), e = avsi_sigmoid(zf[k]);
-            w.u[k] = on ? uf[k] : 0.f;
-            w.delta[k] = on ? d : 0.f;
-            w.slope[k] = on ? (p.softplus ? s : 1.f) : 0.f;
-            w.dy[k] = on ? of[k] * (p.gated ? zf[k] * e : 1.f) : 0.f;
-            w.gz[k] = on ? of[k] * (e * fmaf(zf[k], 1.f - e, 1.f)) : 0.f;
+            const float e = avsi_sigmoid(zf[k]);
+            w.u[k] = uf[k];
+            w.delta[k] = step_size(df[k] + bias[k], p.softplus, w.slope[k]);
+            w.dy[k] = of[k] * (p.gated ? zf[k] * e : 1.f);
+            w.gz[k] = of[k] * (e * fmaf(zf[k], 1.f - e, 1.f));
+        }
+        if (t0 + TT > at.live || at.n < S::CH) {         // (uniform; the sums over channels and time take them all)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool on = st.on[k] && t0 + st.row < at.live;
+                w.u[k] = on ? w.u[k] : 0.f, w.delta[k] = on ? w.delta[k] : 0.f, w.dy[k] = on ? w.dy[k] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
             s_in[buf][st.row][place16<S>(st.row, 4 * st.q + k)] = avsi_f4{w.delta[k], w.delta[k] * w.u[k], w.dy[k], 0.f};
         }
     };
@@ -792,14 +811,18 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
             lane_sums<S>(s_gA[buf], st.row, st.q, gA);
             lane_sums<S>(s_y[buf], st.row, st.q, y);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {           // (behind a length everything held is zero)
+            for (int k = 0; k < 4; ++k) {
                 du[k] = fmaf(Dq[k], w.dy[k], w.delta[k] * gB[k]);
                 ddt[k] = fmaf(w.u[k], gB[k], gA[k]) * w.slope[k];
                 dz[k] = w.gz[k] * fmaf(Dq[k], w.u[k], y[k]);
                 dD[k] = fmaf(w.dy[k], w.u[k], dD[k]);
-                dbias[k] += ddt[k];
-                if (t >= at.live) du[k] = ddt[k] = dz[k] = 0.f;
             }
+            if (t0 + TT > at.live)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (t >= at.live) du[k] = ddt[k] = dz[k] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) dbias[k] += ddt[k];
             put(t0, du, ddt, dz);
         }
     };
