@@ -691,7 +691,6 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
                     }
                     put_part<S>(s_y[buf], t + k, y);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
             float dAt[S::NS] = {};        // (a tile's own sum: the long sum over time keeps its low bits)
 #pragma unroll
@@ -718,7 +717,6 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
                     put_part<S>(s_gA[buf], t, gA);
                     channel_sums<S>(vb, vc, s_bc[buf][threadIdx.x >> 6][t]);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int j = 0; j < S::NS; ++j) dA[j] += dAt[j];
