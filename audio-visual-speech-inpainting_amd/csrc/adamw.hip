@@ -12,6 +12,8 @@
 // copy.  A workgroup takes 4096 consecutive values of one tensor, a wave four blocks of 256, a lane four consecutive values of each:
 // loads of 16 bytes, all of a lane's issued before the first is used.  The tensors of a launch (up to 48) come in its arguments,
 // so nothing is uploaded and a captured launch holds its table; a workgroup finds its tensor by halving over the first chunks.
+// 151 M values, 8-bit moments, bf16 gradients and copies: 475 us (5.1 TB/s, a copy's rate at that size); 4.1 M values in 32 bits: 18.9 us
+// (6.2 TB/s, part of it the Infinity Cache's).
 #include "avsi_common.h"
 #include "avsi_wave.h"
 

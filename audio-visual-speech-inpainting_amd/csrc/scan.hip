@@ -12,8 +12,8 @@
 // Bound: the vector unit.  A state and step costs one exponential (10.5 cycles of its SIMD for a wave, 3.2 for a plain operation) and
 // four (forward) to twelve (backward) plain operations; the bytes of u, dt, z and out come second for N = 16.  A lane owns 4 states
 // of one channel, N / 4 lanes a channel: four independent chains and one exchange of the sum over the states, in LDS.  Time goes by in
-// tiles of 16 steps, between two kinds of waves (below).  8 sequences of 2048 steps and channels, N = 16, bfloat16: forward 169 us
-// (2.4 TB/s with the states it keeps, the vector unit's counter at 81 %), backward 473 us (82 %); one kind of waves that staged, ran and
+// tiles of 16 steps, between two kinds of waves (below).  8 sequences of 2048 steps and channels, N = 16, bfloat16: forward 166 us
+// (2.4 TB/s with the states it keeps, the vector unit's counter at 80 %), backward 463 us (81 %); one kind of waves that staged, ran and
 // wrote in turn took 316 and 770 us.
 //
 // Time is cut into chunks only where batch and channels do not fill the chip (chunks_of): then a first launch runs every chunk from a
@@ -929,8 +929,9 @@ template <typename T> __global__ __launch_bounds__(256) void scan_bc_sum_kernel(
 }
 
 // ---------------------------------------------------------------------------------------------------------- one token
-// Bound by the states, read and written once; a lane's four states of one channel over the sequences b, b + gridDim.y, ..., with the
-// next sequence's operands in flight.  EL: states in no whole quads, one by one.
+// Bound by the states, read and written once (256 sequences of 2048 channels, N = 16: 16 us, 4.9 TB/s).  A lane: four states of one
+// channel, over the sequences b, b + gridDim.y, ..., with the next sequence's operands in flight.  EL: states in no whole quads, one by
+// one.
 template <typename T, int LN, bool EL> __global__ __launch_bounds__(256) void scan_step_kernel(Scan p) {
     const int id = blockIdx.x * 256 + threadIdx.x, ql = id % LN, d = id / LN, n0 = 4 * ql, left = p.N - n0;
     if (d >= p.dim) return;                 // (whole groups of LN lanes leave)
