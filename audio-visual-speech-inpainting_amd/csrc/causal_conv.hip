@@ -6,12 +6,12 @@
 // x[-1], ..., x[1 - K] are the state (the last K - 1 inputs of the piece before, oldest first), or zero.  Behind lengths[b] outputs
 // and gradients are zero, and nothing is read.
 //
-// All of it is bound by memory: one read of x (and dy), one write.  A thread owns 16 bytes of channels and a run of consecutive
+// All of it is bound by memory: one read of x (and dy), one write.  A thread owns four channels and a run of consecutive
 // time steps, which it takes four at a time: the loads of the next four are in flight while these are computed, and the K - 1 inputs in
 // front of them stay in registers, so an input is read once per run and K - 1 inputs again at its start.  In the backward pass the
 // run is followed by K - 1 steps of the next one (dx needs their dpre); the weights' gradients stay in registers over all runs of a
 // thread, are added over a workgroup in LDS and over the workgroups by a second launch, in a fixed order.
-// 8 x 2048 x 2048 bf16, four taps: forward 31 us (4.3 TB/s), backward 54 us (3.7 TB/s) and 5 us for the partials; a copy 5.4 TB/s.
+// 8 x 2048 x 2048 bf16, four taps: forward 28 us (4.8 TB/s), backward 48.5 us (4.2 TB/s) and 5 us for the partials; a copy 5.4 TB/s.
 // Channels in no whole pieces: the last thread takes the last whole piece, which overlaps its neighbour's; both write the same values.
 #include "avsi_common.h"
 #include "avsi_wave.h"
@@ -27,11 +27,9 @@ struct Conv {
     int B, T, D, silu, run;
 };
 
-// Channels of a thread in the forward pass and the step: 16 bytes, or 8 where the windows of more than four taps would not fit the
-// registers.  The backward pass, which holds a second window and the weights' sums, takes four in any type (with eight of 16 bits it
-// ran with one wave per SIMD: 67 against 54.5 us for 16384 x 2048).
-template <typename T, int K> constexpr int channels() { return sizeof(T) == 4 || K > 4 ? 4 : 8; }
-constexpr int BACK = 4;
+// Channels of a thread, in any type.  (Sixteen bytes of a 16-bit type, eight channels, halve the waves that a CU holds: 29.9 against 27.0
+// us forward, 67 against 54 backward, same runs, for 8 x 2048 x 2048 bf16 with four taps.)
+constexpr int V = 4;
 
 __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int T) {
     if (!lengths) return T;
@@ -40,7 +38,7 @@ __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int T) {
 }
 
 // A thread's channels c .. c + V - 1; SMALL: fewer channels than V exist, and they go one by one.
-template <typename T, int V, bool SMALL> struct Lane {
+template <typename T, bool SMALL> struct Lane {
     int c;
     __device__ __forceinline__ Lane(int piece, int D) { c = SMALL ? 0 : (piece * V < D - V ? piece * V : D - V); }
     __device__ __forceinline__ void load(const T* row, int D, avsi_pack<T, V>& v) const {
@@ -71,16 +69,16 @@ template <typename T, int V, bool SMALL> struct Lane {
 };
 
 // Input t of the sequence, 1 - K <= t < 0: from the state, if there is one.
-template <typename T, int K, int V, bool SMALL>
-__device__ __forceinline__ void early(const Conv& a, const Lane<T, V, SMALL>& at, int64_t b, int t, float (&f)[V]) {
+template <typename T, int K, bool SMALL>
+__device__ __forceinline__ void early(const Conv& a, const Lane<T, SMALL>& at, int64_t b, int t, float (&f)[V]) {
     avsi_pack<T, V> v;
     if (a.state) at.load((const T*)a.state + (b * (K - 1) + K - 1 + t) * a.D, a.D, v);
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = a.state ? v.at(i) : 0.f;
 }
 // The K - 1 inputs in front of t0 into x[0 .. K - 2].
-template <typename T, int K, int V, int N, bool SMALL>
-__device__ __forceinline__ void history(const Conv& a, const Lane<T, V, SMALL>& at, const T* xb, int64_t b, int t0, float (&x)[N][V]) {
+template <typename T, int K, int N, bool SMALL>
+__device__ __forceinline__ void history(const Conv& a, const Lane<T, SMALL>& at, const T* xb, int64_t b, int t0, float (&x)[N][V]) {
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
         const int t = t0 - K + 1 + k;
@@ -90,13 +88,13 @@ __device__ __forceinline__ void history(const Conv& a, const Lane<T, V, SMALL>& 
 #pragma unroll
             for (int i = 0; i < V; ++i) x[k][i] = v.at(i);
         } else {
-            early<T, K, V, SMALL>(a, at, b, t, x[k]);
+            early<T, K, SMALL>(a, at, b, t, x[k]);
         }
     }
 }
 
-template <typename T, int K, int V, bool SMALL>
-__device__ __forceinline__ void weights(const Conv& a, const Lane<T, V, SMALL>& at, float (&w)[K][V], float (&bias)[V]) {
+template <typename T, int K, bool SMALL>
+__device__ __forceinline__ void weights(const Conv& a, const Lane<T, SMALL>& at, float (&w)[K][V], float (&bias)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = at.channel(i, a.D);
@@ -107,10 +105,9 @@ __device__ __forceinline__ void weights(const Conv& a, const Lane<T, V, SMALL>& 
 }
 
 template <typename T, int K, bool SMALL> __global__ __launch_bounds__(256) void conv_fwd_kernel(Conv a, int runs) {
-    constexpr int V = channels<T, K>();
     const int nv = (a.D + V - 1) / V;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, rest = id / nv, b = rest / runs;
-    const Lane<T, V, SMALL> at((int)(id % nv), a.D);
+    const Lane<T, SMALL> at((int)(id % nv), a.D);
     const int t0 = (int)(rest % runs) * a.run;
     if (b >= a.B) return;
     const int len = length_of(a.lengths, (int)b, a.T);
@@ -126,8 +123,8 @@ template <typename T, int K, bool SMALL> __global__ __launch_bounds__(256) void 
             for (int j = 0; j < 4; ++j) at.load(xb + (int64_t)(t + j < live ? t + j : live - 1) * a.xt, a.D, next[j]);
         };
         load(t0);
-        weights<T, K, V, SMALL>(a, at, w, bias);
-        history<T, K, V, K + 3, SMALL>(a, at, xb, b, t0, x);
+        weights<T, K, SMALL>(a, at, w, bias);
+        history<T, K, K + 3, SMALL>(a, at, xb, b, t0, x);
         for (int t = t0; t < live; t += 4) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -158,7 +155,7 @@ template <typename T, int K, bool SMALL> __global__ __launch_bounds__(256) void 
     for (int i = 0; i < V; ++i) zero[i] = 0.f;
     for (int t = live > t0 ? live : t0; t < t1; ++t) at.store(yb + (int64_t)t * a.yt, a.D, zero);
     if (a.state_out && t0 == 0) {        // the last K - 1 inputs in front of `len`
-        history<T, K, V, K + 3, SMALL>(a, at, xb, b, len, x);
+        history<T, K, K + 3, SMALL>(a, at, xb, b, len, x);
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) at.store((T*)a.state_out + (b * (K - 1) + k) * a.D, a.D, x[k]);
     }
@@ -167,13 +164,12 @@ template <typename T, int K, bool SMALL> __global__ __launch_bounds__(256) void 
 // part: [gridDim.y][K + 1][D].  A workgroup: `wide` threads along the channels (a power of two), 256 / wide runs.
 template <typename T, int K, bool SMALL>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(Conv a, int runs, int wide, float* __restrict__ part) {
-    constexpr int V = BACK;
     __shared__ float lds[256 * V];
     const int piece = blockIdx.x * wide + threadIdx.x % wide, slot = threadIdx.x / wide, slots = 256 / wide;
     const bool mine = piece * V < a.D;
-    const Lane<T, V, SMALL> at(piece, a.D);
+    const Lane<T, SMALL> at(piece, a.D);
     float w[K][V], bias[V], dw[K][V], db[V];
-    weights<T, K, V, SMALL>(a, at, w, bias);
+    weights<T, K, SMALL>(a, at, w, bias);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         db[i] = 0.f;
@@ -206,7 +202,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(Conv a, int runs, int wid
                     }
                 };
                 load(t0);
-                history<T, K, V, K + 3, SMALL>(a, at, xb, b, t0, x);
+                history<T, K, K + 3, SMALL>(a, at, xb, b, t0, x);
                 for (int t = t0; t < t1 + K - 1; t += 4) {
                     float g[4][V];
 #pragma unroll
@@ -264,7 +260,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(Conv a, int runs, int wid
         __syncthreads();
         for (int i = threadIdx.x; i < wide * V; i += 256) {
             const int of = blockIdx.x * wide + i / V;
-            const int c = Lane<T, V, SMALL>(of, a.D).c + i % V;
+            const int c = Lane<T, SMALL>(of, a.D).c + i % V;
             float s = 0.f;
             for (int j = 0; j < slots; ++j) s += lds[j * wide * V + i];
             if (of * V < a.D && c < a.D) part[((int64_t)blockIdx.y * (K + 1) + k) * a.D + c] = s;
@@ -285,7 +281,6 @@ __global__ __launch_bounds__(1024) void conv_wgrad_sum_kernel(const float* __res
 }
 
 template <typename T, int K> __global__ __launch_bounds__(256) void conv_step_kernel(Conv a) {
-    constexpr int V = channels<T, K>();
     const int nv = (a.D + V - 1) / V;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, b = id / nv;
     if (b >= a.B) return;
@@ -335,21 +330,28 @@ template <typename T, int K> __global__ __launch_bounds__(256) void conv_step_ke
     }
 }
 
-int channels_of(int dtype, int taps) { return dtype == AVSI_F32 || taps > 4 ? 4 : 8; }
-
-// Steps per run, a multiple of four: 4 .. 32, the longest that leaves 2^17 threads (2 waves per SIMD).
-int run_length(int64_t B, int T, int D, int V) {
-    const int64_t r = (B * T * avsi_ceil_div(D, V) >> 17) / 4 * 4;
+// Steps per run, a multiple of four.  Forward: 4 .. 32, the longest that leaves 2^18 threads (4 waves per SIMD).  1 x 8191 x 1536 bf16 in us
+// with 4, 8, 12, 16, 32 steps: 16.5, 14.1, 13.3, 13.2, 14.8 (12 by this rule); 8 x 2048 x 2048: 35.1, 27.6, 27.1, 27.0, 27.6 (32).
+int run_fwd(int64_t B, int T, int D) {
+    const int64_t r = (B * T * avsi_ceil_div(D, V) >> 18) / 4 * 4;
     return (int)(r < 4 ? 4 : r > 32 ? 32 : r);
+}
+// Backward: 8 .. 64, the shortest with which three workgroups to each CU, which is what its registers hold, take all runs at once: a run
+// costs K - 1 more steps, and a fourth workgroup comes after the others.  The same two with 8, 16, 32, 64 steps: 34.0, 26.3, 27.7,
+// 33.3 (16 by this rule) and 64.4, 54.2, 49.6, 45.7 (44: 46).
+constexpr int BACK_WGS = 3 * AVSI_NUM_CU;
+int run_bwd(int64_t B, int T, int D) {
+    const int64_t r = avsi_round_up(avsi_ceil_div(B * T * avsi_ceil_div(D, V), 256 * BACK_WGS), 4);
+    return (int)(r < 8 ? 8 : r > 64 ? 64 : r);
 }
 
 // The backward pass' grid: threads along the channels, and workgroups over the runs = partials of the weights' gradients.
 void bwd_shape(int64_t B, int T, int D, int* wide, int* groups) {
-    const int nv = (int)avsi_ceil_div(D, BACK);
+    const int nv = (int)avsi_ceil_div(D, V);
     *wide = 1;
     while (*wide < 64 && *wide < nv) *wide *= 2;
-    const int64_t runs = B * avsi_ceil_div(T, run_length(B, T, D, BACK)), along = avsi_ceil_div(nv, *wide);
-    int64_t g = avsi_ceil_div(runs, 256 / *wide), most = avsi_ceil_div(4 * AVSI_NUM_CU, along);
+    const int64_t runs = B * avsi_ceil_div(T, run_bwd(B, T, D)), along = avsi_ceil_div(nv, *wide);
+    int64_t g = avsi_ceil_div(runs, 256 / *wide), most = avsi_ceil_div(BACK_WGS, along);
     *groups = (int)(g < most ? g : most);
 }
 
@@ -383,7 +385,7 @@ extern "C" int avsi_causal_conv(const void* x, int64_t x_stride_b, int64_t x_str
                                 int silu, const void* state, const int32_t* lengths, void* y, int64_t y_stride_b, int64_t y_stride_t,
                                 void* state_out, int batch, int time, int dim, int taps, void* stream) {
     if (!shape_ok(dtype, batch, time, dim, taps) || !x || !w || !y) return AVSI_ERR_INVALID_ARG;
-    const int V = channels_of(dtype, taps), run = run_length(batch, time, dim, V), runs = (int)avsi_ceil_div(time, run);
+    const int run = run_fwd(batch, time, dim), runs = (int)avsi_ceil_div(time, run);
     const int64_t wgs = avsi_ceil_div((int64_t)batch * runs * avsi_ceil_div(dim, V), 256);
     if (wgs > 0x7fffffff) return AVSI_ERR_UNSUPPORTED;
     Conv a = {x, nullptr, state, y, state_out, w, bias, lengths, x_stride_b, x_stride_t, y_stride_b, y_stride_t, 0, 0, batch, time, dim, silu, run};
@@ -410,7 +412,7 @@ extern "C" int avsi_causal_conv_bwd(const void* dy, int64_t dy_stride_b, int64_t
         return AVSI_ERR_WORKSPACE;
     int wide, groups;
     bwd_shape(batch, time, dim, &wide, &groups);
-    const int V = BACK, run = run_length(batch, time, dim, V), runs = (int)avsi_ceil_div(time, run);
+    const int run = run_bwd(batch, time, dim), runs = (int)avsi_ceil_div(time, run);
     Conv a = {x, dy, state, dx, nullptr, w, bias, lengths, x_stride_b, x_stride_t, dx_stride_b, dx_stride_t, dy_stride_b, dy_stride_t,
               batch, time, dim, silu, run};
     const dim3 grid(avsi_ceil_div(avsi_ceil_div(dim, V), wide), groups);
@@ -429,11 +431,10 @@ extern "C" int avsi_causal_conv_step(const void* x, int64_t x_stride_b, int dtyp
                                      void* state, void* y, int64_t y_stride_b, int batch, int dim, int taps, void* stream) {
     if (!shape_ok(dtype, batch, 1, dim, taps) || !x || !w || !state || !y) return AVSI_ERR_INVALID_ARG;
     Conv a = {x, nullptr, nullptr, y, state, w, bias, nullptr, x_stride_b, 0, y_stride_b, 0, 0, 0, batch, 1, dim, silu, 1};
-    const int64_t wgs = avsi_ceil_div(batch * avsi_ceil_div(dim, channels_of(dtype, taps)), 256);
+    const int64_t wgs = avsi_ceil_div(batch * avsi_ceil_div(dim, V), 256);
     if (wgs > 0x7fffffff) return AVSI_ERR_UNSUPPORTED;
     avsi_clear_error();
 #define AVSI_GO(T, K, SMALL) hipLaunchKernelGGL((conv_step_kernel<T, K>), dim3(wgs), dim3(256), 0, (hipStream_t)stream, a)
-    const int V = channels_of(dtype, taps);
     AVSI_CONV_T(AVSI_GO)
 #undef AVSI_GO
     return avsi_launch_status();
