@@ -66,7 +66,8 @@ template <int LN_, int NS_, bool EL = false> struct Shape {
     static constexpr int NP = LN * NS;                      // states with their padding
     static constexpr int CH = LN <= 4 ? 64 : 256 / LN;      // channels of a workgroup
     static constexpr int NC = CH * LN, NW = NC / 64;        // consumers: threads, waves
-    static constexpr int QR = CH / 4, PT = QR * TT;         // quads of channels per step; producers: one per quad of a tile
+    static constexpr int QR = CH / 4, PT = 256;             // quads of channels per step; producers
+    static constexpr bool SPARE = PT > QR * TT;             // more of them than quads in a tile: they stage B and C and add dB and dC
     static constexpr int PL = LN > 4 ? 4 : LN;              // parts in which a sum over a channel's lanes is handed to the producers
     static constexpr int QB = NP / 4;                       // quads of states per step
     static constexpr int BPASSES = (TT * QB + PT - 1) / PT;  // of the producers over a tile's [TT][NP] of B and C
@@ -101,10 +102,12 @@ template <typename S> struct Place {
 // masked where it is used.
 template <typename S> struct Stage {
     int id, q, row, c;          // c: the channel (of all) at which the quad is loaded
+    bool works;                 // whether it has a quad of its own (without one it goes through the same steps on another's)
     bool on[4];                 // which of its channels exist
     __device__ __forceinline__ Stage(const Scan& p, const Place<S>& at, int thread) {
         id = thread;
-        q = id % S::QR, row = id / S::QR;
+        q = id % S::QR, row = id / S::QR % TT;
+        works = !S::SPARE || id < S::QR * TT;
         c = at.d0 + 4 * q;
         if (!S::ELEMENTS) c = c < p.dim - 4 ? c : p.dim - 4;
 #pragma unroll
@@ -388,13 +391,14 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
 #pragma unroll
             for (int k = 0; k < 4; ++k) d[k] = on ? d[k] : 0.f, uf[k] = on ? uf[k] : 0.f;
         }
+        if (!st.works) return;
         avsi_f4* to = (avsi_f4*)s_in[buf][st.row];
         to[place8<S>(st.row, 4 * st.q) / 2] = avsi_f4{d[0], d[0] * uf[0], d[1], d[1] * uf[1]};
         to[place8<S>(st.row, 4 * st.q + 2) / 2] = avsi_f4{d[2], d[2] * uf[2], d[3], d[3] * uf[3]};
     };
     auto write = [&](int n, const Held& w) {
         const int t = at.begin + n * TT + st.row;
-        if (t < at.end) {
+        if (t < at.end && st.works) {
             float o[4];
             lane_sums<S>(s_y[n & 1], st.row, st.q, o);
 #pragma unroll
@@ -443,7 +447,9 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
         write(0, even);
     }
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int t0 = at.begin + at.tiles * TT; t0 + st.row < at.end; t0 += TT) put_quad<T>(at_byte(out + t0 * p.ot, place), at.n - 4 * st.q, zero);
+    if (st.works)
+        for (int t0 = at.begin + at.tiles * TT; t0 + st.row < at.end; t0 += TT)
+            put_quad<T>(at_byte(out + t0 * p.ot, place), at.n - 4 * st.q, zero);
 }
 
 // A chunk from a zero state: its end state and the sum of its step sizes.  BACK: the adjoint state, from behind.
@@ -548,6 +554,7 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(S::NC 
 #pragma unroll
             for (int k = 0; k < 4; ++k) d[k] = on ? d[k] : 0.f, x[k] = on ? x[k] : 0.f;
         }
+        if (!st.works) return;
         avsi_f4* to = (avsi_f4*)s_in[buf][st.row];
         to[place8<S>(st.row, 4 * st.q) / 2] = avsi_f4{d[0], x[0], d[1], x[1]};
         to[place8<S>(st.row, 4 * st.q + 2) / 2] = avsi_f4{d[2], x[2], d[3], x[3]};
@@ -786,7 +793,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            s_in[buf][st.row][place16<S>(st.row, 4 * st.q + k)] = avsi_f4{w.delta[k], w.delta[k] * w.u[k], w.dy[k], 0.f};
+            if (st.works) s_in[buf][st.row][place16<S>(st.row, 4 * st.q + k)] = avsi_f4{w.delta[k], w.delta[k] * w.u[k], w.dy[k], 0.f};
         }
     };
     auto finish = [&](int n, const Held& w) {
@@ -803,7 +810,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
                 *(avsi_f2*)(p.part_bc + ((((int64_t)at.b * p.T + t) * p.groups + at.g) * p.blocks + at.block) * ROW + i % ROW) = s;
         }
         const int t = t0 + st.row;
-        if (t < at.end) {
+        if (t < at.end && st.works) {
             float du[4], ddt[4], dz[4], gB[4], gA[4], y[4];
             lane_sums<S>(s_gB[buf], st.row, st.q, gB);
             lane_sums<S>(s_gA[buf], st.row, st.q, gA);
@@ -865,14 +872,16 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
         finish(0, even);
     }
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int t0 = at.begin + at.tiles * TT; t0 + st.row < at.end; t0 += TT) put(t0, zero, zero, zero);
+    if (st.works)
+        for (int t0 = at.begin + at.tiles * TT; t0 + st.row < at.end; t0 += TT) put(t0, zero, zero, zero);
     // D's and the bias' gradients of this workgroup's channels, over its chunk: the rows of the producers
     AVSI_LDS_BARRIER();
+    if (st.works)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        ((float*)s_gB[0][st.row])[4 * st.q + k] = dD[k];
-        ((float*)s_gA[0][st.row])[4 * st.q + k] = dbias[k];
-    }
+        for (int k = 0; k < 4; ++k) {
+            ((float*)s_gB[0][st.row])[4 * st.q + k] = dD[k];
+            ((float*)s_gA[0][st.row])[4 * st.q + k] = dbias[k];
+        }
     AVSI_LDS_BARRIER();
     if (st.id < at.n) {
         float sD = 0.f, sb = 0.f;
