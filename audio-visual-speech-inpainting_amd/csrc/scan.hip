@@ -1010,15 +1010,14 @@ int lanes_of(const avsi_scan_args* a) { return padded(a) / 4; }
 int step_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 int block_channels(int LN) { return LN <= 4 ? 64 : 256 / LN; }
 
-// Chunks of time, of at least 64 steps: as many as give two workgroups to each CU (2048 waves of consumers) and not one more, so that
-// no CU gets a third; none where batch and channels leave one for three of four CUs -- the launch over the chunks costs three quarters
-// of the main one.  2048 steps, N = 16, a whole forward / backward call in us: 2 sequences of 2048 channels (64 workgroups) 146 / 431
+// Chunks of time, of at least 64 steps: as many as give two workgroups to each CU and not one more, so that no CU gets a third; none
+// where batch and channels leave one for three of four CUs -- the launch over the chunks costs three quarters of the main one.  2048 steps, N = 16, a whole forward / backward call in us: 2 sequences of 2048 channels (64 workgroups) 146 / 431
 // uncut, 67 / 158 in 8 chunks (85 / 204 in 6, 79 / 188 in 10); 4 (128) 147 / 439 uncut, 120 / 291 in 4; 6 (192) 152 / 445 uncut,
-// 185 / 514 in 2, 175 / 428 in 4.
+// 185 / 514 in 2, 175 / 428 in 4.  Fewer states make smaller workgroups, but no more of them: 8191 steps of 1536 channels with 4 / 8
+// states in 21 chunks 75 / 217 and 94 / 226; in as many as make the waves of 16 states, 85 and 42, 83 / 236 and 98 / 242.
 void chunks_of(const avsi_scan_args* a, int* chunk, int* chunks) {
-    const int LN = lanes_of(a), CH = block_channels(LN);
-    const int64_t waves = (int64_t)a->batch * a->groups * avsi_ceil_div(a->dim / a->groups, CH) * (CH * LN / 64);
-    int64_t n = waves >= 768 ? 1 : 2048 / waves;
+    const int64_t wgs = (int64_t)a->batch * a->groups * avsi_ceil_div(a->dim / a->groups, block_channels(lanes_of(a)));
+    int64_t n = wgs >= 3 * AVSI_NUM_CU / 4 ? 1 : 2 * AVSI_NUM_CU / wgs;
     const int64_t most = avsi_ceil_div(a->time, 64);
     n = n < most ? n : most;
     *chunk = (int)avsi_round_up(avsi_ceil_div(a->time, n), TT);
