@@ -355,9 +355,9 @@ void bwd_shape(int64_t B, int T, int D, int* wide, int* groups) {
     *groups = (int)(g < most ? g : most);
 }
 
-// (time up to 2^30: a step in front of or behind a sequence still has a number)
+// (time up to 2^30: a step in front of or behind a sequence still has a number; channels likewise, behind the last one)
 bool shape_ok(int dtype, int B, int T, int D, int taps) {
-    return avsi_dtype_ok(dtype) && B > 0 && T > 0 && T <= (1 << 30) && D > 0 && taps >= 2 && taps <= 8;
+    return avsi_dtype_ok(dtype) && B > 0 && T > 0 && T <= (1 << 30) && D > 0 && D <= 0x7fffffff - 1023 && taps >= 2 && taps <= 8;
 }
 
 }  // namespace

@@ -10,9 +10,18 @@ from . import _lib
 
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
+# Largest sizes, those that the C entry points state.  They are checked here, before anything is allocated: the entry points take sizes
+# in 32 bits, and ctypes cuts a larger number without a word.
+_MOST = {"columns": 1 << 30, "steps": 1 << 30, "scan channels": 1 << 26, "channels": (1 << 31) - 1024, "sequences": (1 << 31) - 1}
+
 
 def _bad(what, *args):
     raise _lib.AvsiError(what % args)
+
+
+def _fits(what, size, n):
+    if n > _MOST[size]:
+        _bad("%s: at most %d %s, not %d", what, _MOST[size], size.split()[-1], n)
 
 
 def _device(what, first, *others):
@@ -44,6 +53,7 @@ def _rows(what, name, t, cols=None):
     if t.dtype not in _CODES or t.dim() < 1:
         _bad("%s: %s must be a float32, bfloat16 or float16 tensor", what, name)
     C = t.shape[-1]
+    _fits(what, "columns", C)
     if cols is not None and C != cols:
         _bad("%s: %s has %d columns, not %d", what, name, C, cols)
     if t.dim() == 2:
@@ -165,6 +175,10 @@ def _conv_args(what, x, w, bias, dims):
     if x.dtype not in _CODES or x.dim() != dims:
         _bad("%s: x must be a float32, bfloat16 or float16 tensor of %d dimensions", what, dims)
     D = x.shape[-1]
+    _fits(what, "sequences", x.shape[0])
+    _fits(what, "channels", D)
+    if dims == 3:
+        _fits(what, "steps", x.shape[1])
     if w.dim() != 2 or not 2 <= w.shape[1] <= 8 or D < 1:
         _bad("%s: w must be [channels, taps] with 2 to 8 taps", what)
     _vector(what, "w", w, D, w.shape[1])
@@ -256,6 +270,9 @@ def _scan_operands(what, u, dt, A, B, C, D, z, dt_bias, softplus):
     lead, dim, two = shape[:-1], shape[-1], len(shape) == 3
     if dtype not in _CODES or dim < 1:
         _bad("%s: u must be a float32, bfloat16 or float16 tensor with channels", what)
+    _fits(what, "scan channels", dim)
+    if two:
+        _fits(what, "steps", lead[1])
     if A.dim() != 2 or not 1 <= A.shape[1] <= 64:
         _bad("%s: A must be [channels, states] with 1 to 64 states", what)
     N = A.shape[1]

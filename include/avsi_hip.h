@@ -711,6 +711,7 @@ int avsi_tfrecord_files_decode_fixed_host(const char* const* paths, int count, i
  *   y = h gamma + beta;   e = dy gamma, dx = rstd (e - mean(e) - h mean(e h)), dgamma = sum_rows dy h, dbeta = sum_rows dy.
  *   x, y, dy, dx  elements of type `dtype` (avsi_dtype), unit stride along a row, row strides in elements, any alignment
  *                 an element has; every output tensor distinct from the inputs
+ *   cols          at most 2^30
  *   gamma, beta   [cols] of type `wdtype` (AVSI_F32, or the same as dtype); either may be NULL (1 and 0)
  *   mean, rstd    [rows] float; dgamma, dbeta [cols] float, both NULL when they are not wanted
  * All sums are fp32; outputs are rounded once, to nearest even.  The reduction over the rows is deterministic: partials
@@ -733,7 +734,7 @@ int avsi_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_
  *   w [dim][taps], bias [dim] (or NULL), dw, dbias: float
  *   state          `dtype` [batch][taps - 1][dim]: the inputs in front of x[0], oldest first; NULL: zeros.  It is a
  *                  constant of the backward pass
- *   time           at most 2^30
+ *   time           at most 2^30; dim at most 2^31 - 1024
  *   lengths        device int32 [batch] or NULL: sequence b has min(max(lengths[b], 0), time) steps; behind them y and dx
  *                  are zero and x, dy are not read
  *   state_out      `dtype` [batch][taps - 1][dim] or NULL: the last inputs in front of each sequence's end (not `state`)
