@@ -153,32 +153,42 @@ template <int G, typename OP = avsi_add> __device__ __forceinline__ float avsi_g
     return v;
 }
 
-// Column c = 32 blockIdx.x + (threadIdx.x & 31) of P rows of partials, added by a workgroup of 1024: 32 slices of the rows, eight loads
-// of a slice in flight, then the slices, all in a fixed order.  The sum is in the first 32 threads.
-__device__ __forceinline__ float avsi_column_sum(const float* __restrict__ part, int P, int64_t stride, int64_t cols) {
+// Sums of P rows of partials by columns, handed to `put(column, sum)`, by workgroups of 1024 in a grid of avsi_column_sum_grid(cols):
+// 32 columns at a time in 32 slices of the rows, eight loads of a slice in flight, then the slices, all in a fixed order.
+// (A launch has fewer than 2^32 threads: of more than 2^26 columns a workgroup takes several blocks.)
+static inline dim3 avsi_column_sum_grid(int64_t cols) {
+    const int64_t blocks = (cols + 31) / 32, most = 1 << 21;
+    return dim3((unsigned)(blocks < most ? blocks : most));
+}
+template <typename Put> __device__ __forceinline__ void avsi_column_sums(const float* __restrict__ part, int P, int64_t stride, int64_t cols,
+                                                                         Put put) {
     __shared__ float lds[32][33];
-    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int slice = threadIdx.x >> 5;
-    float s = 0.f;
-    if (c < cols) {
-        const float* at = part + c;
-        int r = slice;
-        for (; r + 7 * 32 < P; r += 8 * 32) {
-            float v[8];
+    const int slice = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < cols; c0 += (int64_t)gridDim.x * 32) {
+        const int64_t c = c0 + lane;
+        float s = 0.f;
+        if (c < cols) {
+            const float* at = part + c;
+            int r = slice;
+            for (; r + 7 * 32 < P; r += 8 * 32) {
+                float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = at[(int64_t)(r + 32 * i) * stride];
+                for (int i = 0; i < 8; ++i) v[i] = at[(int64_t)(r + 32 * i) * stride];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[i];
+                for (int i = 0; i < 8; ++i) s += v[i];
+            }
+            for (; r < P; r += 32) s += at[(int64_t)r * stride];
         }
-        for (; r < P; r += 32) s += at[(int64_t)r * stride];
-    }
-    lds[slice][threadIdx.x & 31] = s;
-    __syncthreads();
-    s = 0.f;
-    if (threadIdx.x < 32)
+        if (c0 != (int64_t)blockIdx.x * 32) __syncthreads();        // (the block before has been read)
+        lds[slice][lane] = s;
+        __syncthreads();
+        if (threadIdx.x < 32 && c < cols) {
+            s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s += lds[i][threadIdx.x];
-    return s;
+            for (int i = 0; i < 32; ++i) s += lds[i][lane];
+            put(c, s);
+        }
+    }
 }
 
 // Functions of the gates, to a few ulp, on the hardware's base-2 exponential.  In softplus x log2 e is carried in two words; then

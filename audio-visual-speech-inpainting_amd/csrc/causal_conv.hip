@@ -271,13 +271,12 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(Conv a, int runs, int wid
 // dw[d][k], dbias[d] = sums of part[P][K + 1][D].
 __global__ __launch_bounds__(1024) void conv_wgrad_sum_kernel(const float* __restrict__ part, int P, int K, int D, float* __restrict__ dw,
                                                               float* __restrict__ dbias) {
-    const int64_t cols = (int64_t)(K + 1) * D, c = (int64_t)blockIdx.x * 32 + threadIdx.x;
-    const float s = avsi_column_sum(part, P, cols, cols);
-    if (threadIdx.x < 32 && c < cols) {
+    const int64_t cols = (int64_t)(K + 1) * D;
+    avsi_column_sums(part, P, cols, cols, [&](int64_t c, float s) {
         const int k = (int)(c / D), d = (int)(c % D);
         if (k < K) dw[(int64_t)d * K + k] = s;
         else if (dbias) dbias[d] = s;
-    }
+    });
 }
 
 template <typename T, int K> __global__ __launch_bounds__(256) void conv_step_kernel(Conv a) {
@@ -422,7 +421,7 @@ extern "C" int avsi_causal_conv_bwd(const void* dy, int64_t dy_stride_b, int64_t
     AVSI_CONV_T(AVSI_GO)
 #undef AVSI_GO
     if (dw)
-        hipLaunchKernelGGL(conv_wgrad_sum_kernel, dim3(avsi_ceil_div((int64_t)(taps + 1) * dim, 32)), dim3(1024), 0, (hipStream_t)stream,
+        hipLaunchKernelGGL(conv_wgrad_sum_kernel, avsi_column_sum_grid((int64_t)(taps + 1) * dim), dim3(1024), 0, (hipStream_t)stream,
                            part, groups, taps, dim, dw, dbias);
     return avsi_launch_status();
 }

@@ -362,12 +362,10 @@ __global__ __launch_bounds__(256) void ln_wgrad_wide_kernel(const T* __restrict_
 // dgamma, dbeta = sums of part[P][2][C].
 __global__ __launch_bounds__(1024) void ln_wgrad_sum_kernel(const float* __restrict__ part, int P, int C, float* __restrict__ dgamma,
                                                             float* __restrict__ dbeta) {
-    const float s = avsi_column_sum(part, P, 2 * (int64_t)C, 2 * (int64_t)C);
-    const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
-    if (threadIdx.x < 32 && c < 2 * (int64_t)C) {
+    avsi_column_sums(part, P, 2 * (int64_t)C, 2 * (int64_t)C, [&](int64_t c, float s) {
         if (c < C) dgamma[c] = s;
         else dbeta[c - C] = s;
-    }
+    });
 }
 
 // The group of lanes that a row of C columns takes, and its pieces per lane; 0 lanes: none holds it.  Four pieces only in the
@@ -451,7 +449,7 @@ int launch_bwd(const void* dy, int64_t dys, const void* x, int64_t xs, const flo
 #undef AVSI_LN_BWD_W
 #undef AVSI_LN_BWD
     if (dgamma)
-        hipLaunchKernelGGL(ln_wgrad_sum_kernel, dim3(avsi_ceil_div(2 * (int64_t)C, 32)), dim3(1024), 0, s, part, P, C, dgamma, dbeta);
+        hipLaunchKernelGGL(ln_wgrad_sum_kernel, avsi_column_sum_grid(2 * (int64_t)C), dim3(1024), 0, s, part, P, C, dgamma, dbeta);
     return avsi_launch_status();
 }
 

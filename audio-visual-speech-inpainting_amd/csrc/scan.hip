@@ -899,9 +899,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
 // dA [dim][N], dD, ddt_bias [dim] = sums over P partials of [dim][NP], [dim], [dim].
 __global__ __launch_bounds__(1024) void scan_wgrad_sum_kernel(const float* __restrict__ part, int P, int dim, int NP, int N,
                                                               float* __restrict__ dA, float* __restrict__ dD, float* __restrict__ dbias) {
-    const int64_t cols = (int64_t)dim * (NP + 2), c = (int64_t)blockIdx.x * 32 + threadIdx.x;
-    const float s = avsi_column_sum(part, P, partial_stride(dim, NP), cols);
-    if (threadIdx.x < 32 && c < cols) {
+    avsi_column_sums(part, P, partial_stride(dim, NP), (int64_t)dim * (NP + 2), [&](int64_t c, float s) {
         if (c < (int64_t)dim * NP) {
             if (c % NP < N) dA[c / NP * N + c % NP] = s;
         } else if (c < (int64_t)dim * (NP + 1)) {
@@ -909,14 +907,15 @@ __global__ __launch_bounds__(1024) void scan_wgrad_sum_kernel(const float* __res
         } else if (dbias) {
             dbias[c - (int64_t)dim * (NP + 1)] = s;
         }
-    }
+    });
 }
 
 // dB, dC [batch][time][groups][N] = sums over the blocks of part_bc; zero behind a length.  A thread: four states of one of the two,
-// the partials of eight blocks in flight.
-template <typename T> __global__ __launch_bounds__(256) void scan_bc_sum_kernel(Scan p, int NP, T* __restrict__ dB, T* __restrict__ dC) {
+// the partials of eight blocks in flight.  `first`: where this launch begins (one has fewer than 2^32 threads).
+template <typename T>
+__global__ __launch_bounds__(256) void scan_bc_sum_kernel(Scan p, int NP, int64_t first, T* __restrict__ dB, T* __restrict__ dC) {
     const int Q = NP / 2;                   // quads of dB and dC of a token and group
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, tg = id / Q;
+    const int64_t id = first + (int64_t)blockIdx.x * 256 + threadIdx.x, tg = id / Q;
     if (tg >= (int64_t)p.batch * p.T * p.groups) return;
     const int q = (int)(id % Q), n = 4 * (q % (NP / 4)), t = (int)(tg / p.groups % p.T), b = (int)(tg / p.groups / p.T);
     if (n >= p.N) return;
@@ -1160,15 +1159,17 @@ extern "C" int avsi_selective_scan_bwd(const avsi_scan_args* a, void* workspace,
     hipStream_t s = (hipStream_t)stream;
     avsi_clear_error();
     AVSI_SCAN_T(AVSI_SCAN_N, go_bwd)
-    const int64_t bc = (int64_t)p.batch * p.T * p.groups * NP / 2;
-    const dim3 grid(avsi_ceil_div(bc, 256));
-    if (a->dtype == AVSI_F32)
-        hipLaunchKernelGGL((scan_bc_sum_kernel<float>), grid, dim3(256), 0, s, p, NP, (float*)a->dB, (float*)a->dC);
-    else if (a->dtype == AVSI_BF16)
-        hipLaunchKernelGGL((scan_bc_sum_kernel<__bf16>), grid, dim3(256), 0, s, p, NP, (__bf16*)a->dB, (__bf16*)a->dC);
-    else
-        hipLaunchKernelGGL((scan_bc_sum_kernel<_Float16>), grid, dim3(256), 0, s, p, NP, (_Float16*)a->dB, (_Float16*)a->dC);
-    hipLaunchKernelGGL(scan_wgrad_sum_kernel, dim3(avsi_ceil_div((int64_t)p.dim * (NP + 2), 32)), dim3(1024), 0, s, p.part_w,
+    const int64_t bc = (int64_t)p.batch * p.T * p.groups * NP / 2, most = (int64_t)1 << 31;
+    for (int64_t first = 0; first < bc; first += most) {
+        const dim3 grid((unsigned)avsi_ceil_div(bc - first < most ? bc - first : most, 256));
+        if (a->dtype == AVSI_F32)
+            hipLaunchKernelGGL((scan_bc_sum_kernel<float>), grid, dim3(256), 0, s, p, NP, first, (float*)a->dB, (float*)a->dC);
+        else if (a->dtype == AVSI_BF16)
+            hipLaunchKernelGGL((scan_bc_sum_kernel<__bf16>), grid, dim3(256), 0, s, p, NP, first, (__bf16*)a->dB, (__bf16*)a->dC);
+        else
+            hipLaunchKernelGGL((scan_bc_sum_kernel<_Float16>), grid, dim3(256), 0, s, p, NP, first, (_Float16*)a->dB, (_Float16*)a->dC);
+    }
+    hipLaunchKernelGGL(scan_wgrad_sum_kernel, avsi_column_sum_grid((int64_t)p.dim * (NP + 2)), dim3(1024), 0, s, p.part_w,
                        p.batch * p.chunks, p.dim, NP, p.N, a->dA, a->dD, a->ddt_bias);
     return avsi_launch_status();
 }
