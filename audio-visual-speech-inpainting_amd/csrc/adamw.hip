@@ -22,6 +22,7 @@ namespace {
 constexpr int MOST = 48;                // tensors per launch: their table and the rest of the arguments stay below 4 KiB
 constexpr int BLOCK = 256, PER_LANE = 4;
 constexpr int CHUNK = 4 * PER_LANE * BLOCK;       // values of a workgroup
+constexpr int64_t LAUNCH = ((int64_t)1 << 24) - 1;       // workgroups of a launch, which has fewer than 2^32 threads
 
 struct Table {
     avsi_adamw_tensor t[MOST];
@@ -177,7 +178,7 @@ extern "C" int avsi_adamw(const avsi_adamw_tensor* tensors, int count, int bits,
         return AVSI_ERR_INVALID_ARG;
     for (int i = 0; i < count; ++i) {
         const avsi_adamw_tensor& t = tensors[i];
-        if (t.numel < 0 || t.numel > ((int64_t)1 << 40)) return AVSI_ERR_INVALID_ARG;
+        if (t.numel < 0 || t.numel > LAUNCH * CHUNK) return AVSI_ERR_INVALID_ARG;
         if (t.numel == 0) continue;
         if (!t.w || !t.grad || !t.m || !t.v || !avsi_dtype_ok(t.grad_dtype) || (t.copy && !avsi_dtype_ok(t.copy_dtype)) ||
             (bits == 8 && (!t.m_scale || !t.v_scale)))
@@ -194,7 +195,7 @@ extern "C" int avsi_adamw(const avsi_adamw_tensor* tensors, int count, int bits,
     int64_t chunks = 0;
     for (int i = 0; i <= count; ++i) {
         const int64_t more = i < count ? avsi_ceil_div(tensors[i].numel, CHUNK) : 0;
-        if (tab.count && (i == count || tab.count == MOST || chunks + more > 0x7fffffff)) {
+        if (tab.count && (i == count || tab.count == MOST || chunks + more > LAUNCH)) {
             if (bits == 32) hipLaunchKernelGGL(adamw_kernel<32>, dim3(chunks), dim3(256), 0, (hipStream_t)stream, tab, h);
             else hipLaunchKernelGGL(adamw_kernel<8>, dim3(chunks), dim3(256), 0, (hipStream_t)stream, tab, h);
             tab.count = 0;

@@ -18,6 +18,9 @@ static inline int avsi_launch_status() {
 static inline int64_t avsi_ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t avsi_round_up(int64_t a, int64_t b) { return avsi_ceil_div(a, b) * b; }
 
+// Whether a launch of `wgs` workgroups of `threads` is one that the runtime takes: fewer than 2^32 threads along x.
+static inline bool avsi_grid_ok(int64_t wgs, int threads) { return wgs < (((int64_t)1 << 32) + threads - 1) / threads; }
+
 // MI355X: 256 CUs in 8 XCDs.  Used only to size persistent grids.
 #define AVSI_NUM_CU 256
 #define AVSI_NUM_XCD 8

@@ -386,7 +386,7 @@ extern "C" int avsi_causal_conv(const void* x, int64_t x_stride_b, int64_t x_str
     if (!shape_ok(dtype, batch, time, dim, taps) || !x || !w || !y) return AVSI_ERR_INVALID_ARG;
     const int run = run_fwd(batch, time, dim), runs = (int)avsi_ceil_div(time, run);
     const int64_t wgs = avsi_ceil_div((int64_t)batch * runs * avsi_ceil_div(dim, V), 256);
-    if (wgs > 0x7fffffff) return AVSI_ERR_UNSUPPORTED;
+    if (!avsi_grid_ok(wgs, 256)) return AVSI_ERR_UNSUPPORTED;
     Conv a = {x, nullptr, state, y, state_out, w, bias, lengths, x_stride_b, x_stride_t, y_stride_b, y_stride_t, 0, 0, batch, time, dim, silu, run};
     avsi_clear_error();
 #define AVSI_GO(T, K, SMALL) hipLaunchKernelGGL((conv_fwd_kernel<T, K, SMALL>), dim3(wgs), dim3(256), 0, (hipStream_t)stream, a, runs)
@@ -431,7 +431,7 @@ extern "C" int avsi_causal_conv_step(const void* x, int64_t x_stride_b, int dtyp
     if (!shape_ok(dtype, batch, 1, dim, taps) || !x || !w || !state || !y) return AVSI_ERR_INVALID_ARG;
     Conv a = {x, nullptr, nullptr, y, state, w, bias, nullptr, x_stride_b, 0, y_stride_b, 0, 0, 0, batch, 1, dim, silu, 1};
     const int64_t wgs = avsi_ceil_div(batch * avsi_ceil_div(dim, V), 256);
-    if (wgs > 0x7fffffff) return AVSI_ERR_UNSUPPORTED;
+    if (!avsi_grid_ok(wgs, 256)) return AVSI_ERR_UNSUPPORTED;
     avsi_clear_error();
 #define AVSI_GO(T, K, SMALL) hipLaunchKernelGGL((conv_step_kernel<T, K>), dim3(wgs), dim3(256), 0, (hipStream_t)stream, a)
     AVSI_CONV_T(AVSI_GO)

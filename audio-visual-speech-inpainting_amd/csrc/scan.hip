@@ -1028,6 +1028,9 @@ bool shape_ok(const avsi_scan_args* a) {
            a->dim <= (1 << 26) && a->state > 0 && a->groups > 0 && a->dim % a->groups == 0;
 }
 
+// The workgroups of a sequence, of 16 channels of a group or more and up to 512 threads, are one launch.
+bool grid_ok(const avsi_scan_args* a) { return avsi_grid_ok(a->groups * avsi_ceil_div(a->dim / a->groups, 16), 512); }
+
 // A tile's rows are addressed with 32 bits from its first one.  (A single step has no second row: any stride will do.)
 bool strides_ok(const avsi_scan_args* a) {
     if (a->time == 1) return true;
@@ -1123,7 +1126,7 @@ extern "C" size_t avsi_selective_scan_workspace_bytes(const avsi_scan_args* a) {
 
 extern "C" int avsi_selective_scan(const avsi_scan_args* a, void* workspace, size_t workspace_bytes, void* stream) {
     if (!shape_ok(a) || !a->u || !a->dt || !a->A || !a->B || !a->C || !a->out) return AVSI_ERR_INVALID_ARG;
-    if (a->state > MAX_STATE || !strides_ok(a)) return AVSI_ERR_UNSUPPORTED;
+    if (a->state > MAX_STATE || !strides_ok(a) || !grid_ok(a)) return AVSI_ERR_UNSUPPORTED;
     const size_t need = avsi_selective_scan_workspace_bytes(a);
     if (need && (!workspace || workspace_bytes < need)) return AVSI_ERR_WORKSPACE;
     Scan p = params(a);
@@ -1147,7 +1150,7 @@ extern "C" int avsi_selective_scan_bwd(const avsi_scan_args* a, void* workspace,
     if (!shape_ok(a) || !a->u || !a->dt || !a->A || !a->B || !a->C || !a->dout || !a->kept || !a->du || !a->ddt || !a->dA || !a->dB ||
         !a->dC || !a->z != !a->dz)
         return AVSI_ERR_INVALID_ARG;
-    if (a->state > MAX_STATE || !strides_ok(a)) return AVSI_ERR_UNSUPPORTED;
+    if (a->state > MAX_STATE || !strides_ok(a) || !grid_ok(a)) return AVSI_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < avsi_selective_scan_bwd_workspace_bytes(a)) return AVSI_ERR_WORKSPACE;
     Scan p = params(a);
     const int NP = p.NP;

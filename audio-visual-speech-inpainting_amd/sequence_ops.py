@@ -296,6 +296,8 @@ def _scan_operands(what, u, dt, A, B, C, D, z, dt_bias, softplus):
     G2, sC = _groups(what, "C", C, lead, N, dtype)
     if G != G2 or G < 1 or dim % G:
         _bad("%s: B and C must have one number of groups, which divides the %d channels", what, dim)
+    if two and G * -(-(dim // G) // 16) >= 1 << 23:
+        _bad("%s: groups * ceil(channels / groups / 16) has to be below 2^23", what)
     t = (lambda s: s[1]) if two else (lambda s: 0)
     return N, (_CODES[dtype], lead[0], lead[1] if two else 1, dim, N, G, int(softplus), 0, u.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(),
                C.data_ptr(), su[0], t(su), sd[0], t(sd), sz[0], t(sz), *sB, *sC, A.data_ptr(), _p(D), _p(dt_bias))

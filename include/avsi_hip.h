@@ -734,7 +734,8 @@ int avsi_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_
  *   w [dim][taps], bias [dim] (or NULL), dw, dbias: float
  *   state          `dtype` [batch][taps - 1][dim]: the inputs in front of x[0], oldest first; NULL: zeros.  It is a
  *                  constant of the backward pass
- *   time           at most 2^30; dim at most 2^31 - 1024
+ *   time           at most 2^30; dim at most 2^31 - 1024; forward and step: fewer than 2^32 threads, one per four channels and
+ *                  run of time (4 .. 32 steps, the more the larger batch * time * dim)
  *   lengths        device int32 [batch] or NULL: sequence b has min(max(lengths[b], 0), time) steps; behind them y and dx
  *                  are zero and x, dy are not read
  *   state_out      `dtype` [batch][taps - 1][dim] or NULL: the last inputs in front of each sequence's end (not `state`)
@@ -760,7 +761,8 @@ int avsi_causal_conv_step(const void* x, int64_t x_stride_b, int dtype, const fl
  *   B, C             `dtype` [batch][time][groups][state], strides {batch, time, group}, unit stride along the states;
  *                    channel d belongs to group d / (dim / groups)
  *   A [dim][state], D [dim] or NULL (0), dt_bias [dim] or NULL (0): float.  state <= 64, batch <= 65535,
- *                    time <= 2^30, dim <= 2^26; strides of time from 0 to 2^26 unless time is 1
+ *                    time <= 2^30, dim <= 2^26; strides of time from 0 to 2^26 unless time is 1; except for the step,
+ *                    groups * ceil(dim / groups / 16) < 2^23
  *   state_in         float [batch][dim][state] or NULL (zeros), a constant of the backward pass; state_out: the state at each
  *                    sequence's end, or NULL (not state_in)
  *   lengths          as for the convolution: behind its length a sequence's state stands still, out and all gradients are
@@ -804,7 +806,8 @@ int avsi_selective_scan_step(const avsi_scan_args* args, void* stream);
  *   bits 32: m, v float.  bits 8: one byte per value, e4m3 codes of m / m_scale and of sqrt(v) / v_scale, where block k of
  *   256 consecutive values of a tensor has the scales m_scale[k] = max|m| / 448, v_scale[k] = max sqrt(v) / 448; a value of
  *   v above zero keeps at least the code of 2^-9.  A block that holds a non-finite moment decodes to NaN.
- * `tensors` is a HOST array (read during the call, its pointers are device pointers; numel 0 is skipped); the tensors must
+ * `tensors` is a HOST array (read during the call, its pointers are device pointers; numel 0 is skipped, at most
+ * 2^36 - 2^12); the tensors must
  * not share memory.  `skip` as for avsi_adam_tf_guarded_f32: with any of its words non-zero nothing is written.
  * ------------------------------------------------------------------------------------ */
 typedef struct avsi_adamw_tensor {
