@@ -571,6 +571,8 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(S::NC 
 }
 
 // start[c] = local end of c - 1 + exp(A sum of c - 1) start[c - 1] (BACK: with c + 1), in place.  One thread per four states.
+// The exponential of a whole chunk may leave the range of a float where the states, which its steps multiply one by one, do not
+// (growth from zero or a tiny state, an infinite one that decays): its power of two goes onto the state by itself.
 template <bool BACK> __global__ __launch_bounds__(256) void scan_join_kernel(Scan p, int QB) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= (int64_t)p.batch * p.dim * QB) return;
@@ -599,7 +601,10 @@ template <bool BACK> __global__ __launch_bounds__(256) void scan_join_kernel(Sca
         for (int k = 0; k < 8; ++k)
             if (i0 + k < p.chunks) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[k][j] = h[j] = fmaf(__builtin_amdgcn_exp2f(sum[k] * A[j]), h[j], v[k][j]);
+                for (int j = 0; j < 4; ++j) {
+                    const float x = fmaxf(fminf(sum[k] * A[j], 1000.f), -1000.f), n = floorf(x);     // (2^+-1000 takes any state to its end)
+                    v[k][j] = h[j] = fmaf(__builtin_amdgcn_exp2f(x - n), ldexpf(h[j], (int)n), v[k][j]);
+                }
                 *(avsi_f4*)(p.ends + (row(i0 + k) * QB + ql) * 4) = v[k];
             }
     }
