@@ -222,12 +222,16 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(Conv a, int runs, int wid
 #pragma unroll
                             for (int k = 0; k < K; ++k) p = fmaf(w[k][i], x[j + k][i], p);
                             const float s = avsi_sigmoid(p), slope = s * fmaf(p, 1.f - s, 1.f);
-                            const float e = live ? g[j][i] * (a.silu ? slope : 1.f) : 0.f, mineonly = own ? e : 0.f;
-                            d[K - 1 + j][i] = e;
-                            db[i] += mineonly;
-#pragma unroll
-                            for (int k = 0; k < K; ++k) dw[k][i] = fmaf(mineonly, x[j + k][i], dw[k][i]);
+                            d[K - 1 + j][i] = live ? g[j][i] * (a.silu ? slope : 1.f) : 0.f;
                         }
+                        // (not with a factor of zero: an input that is infinite or NaN belongs to the steps that it is a tap of)
+                        if (own)
+#pragma unroll
+                            for (int i = 0; i < V; ++i) {
+                                db[i] += d[K - 1 + j][i];
+#pragma unroll
+                                for (int k = 0; k < K; ++k) dw[k][i] = fmaf(d[K - 1 + j][i], x[j + k][i], dw[k][i]);
+                            }
                         float o[V];
 #pragma unroll
                         for (int i = 0; i < V; ++i) {
