@@ -139,7 +139,7 @@ template <typename T, int K, bool SMALL> __global__ __launch_bounds__(256) void 
                     float p = bias[i];
 #pragma unroll
                     for (int k = 0; k < K; ++k) p = fmaf(w[k][i], x[j + k][i], p);
-                    const float s = p * avsi_sigmoid(p);
+                    const float s = p * avsi_sigmoid<T>(p);
                     o[i] = a.silu ? s : p;
                 }
                 if (t + j < live) at.store(yb + (int64_t)(t + j) * a.yt, a.D, o);
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(Conv a, int runs, int wid
                             float p = bias[i];
 #pragma unroll
                             for (int k = 0; k < K; ++k) p = fmaf(w[k][i], x[j + k][i], p);
-                            const float s = avsi_sigmoid(p), slope = s * fmaf(p, 1.f - s, 1.f);
+                            const float s = avsi_sigmoid<T>(p), slope = s * fmaf(p, 1.f - s, 1.f);
                             d[K - 1 + j][i] = live ? g[j][i] * (a.silu ? slope : 1.f) : 0.f;
                         }
                         // (not with a factor of zero: an input that is infinite or NaN belongs to the steps that it is a tap of)
@@ -314,7 +314,7 @@ template <typename T, int K> __global__ __launch_bounds__(256) void conv_step_ke
         float p = a.bias ? a.bias[ch] : 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k) p = fmaf(a.w[(int64_t)ch * K + k], win[k].at(i), p);
-        const float s = p * avsi_sigmoid(p);
+        const float s = p * avsi_sigmoid<T>(p);
         o[i] = a.silu ? s : p;
     }
     T* y = (T*)a.y + b * a.yb + c;

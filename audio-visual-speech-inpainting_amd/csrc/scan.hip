@@ -381,7 +381,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
         float d[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float g = zf[k] * avsi_sigmoid(zf[k]);
+            const float g = zf[k] * avsi_sigmoid<T>(zf[k]);
             d[k] = step_size(df[k] + bias[k], p.softplus);
             w.thru[k] = Dq[k] * uf[k];
             w.gate[k] = p.gated ? g : 1.f;
@@ -546,7 +546,7 @@ template <typename T, typename S, bool BACK> __global__ __launch_bounds__(S::NC 
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             d[k] = step_size(df[k] + bias[k], p.softplus);
-            const float gate = zf[k] * avsi_sigmoid(zf[k]);
+            const float gate = zf[k] * avsi_sigmoid<T>(zf[k]);
             x[k] *= BACK ? (p.gated ? gate : 1.f) : d[k];
         }
         if (t0 + TT > at.live) {
@@ -783,7 +783,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NC + S::PT) vo
         const int t0 = tile_at(n), buf = n & 1;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float e = avsi_sigmoid(zf[k]);
+            const float e = avsi_sigmoid<T>(zf[k]);
             w.u[k] = uf[k];
             w.delta[k] = step_size(df[k] + bias[k], p.softplus, w.slope[k]);
             w.dy[k] = of[k] * (p.gated ? zf[k] * e : 1.f);
@@ -997,7 +997,7 @@ template <typename T, int LN, bool EL> __global__ __launch_bounds__(256) void sc
         y = avsi_group<LN>(y);
         if (ql == 0) {
             y = fmaf(Dd, uf, y);
-            ((T*)p.out)[b * p.ob + d] = (T)(p.gated ? y * (zf * avsi_sigmoid(zf)) : y);
+            ((T*)p.out)[b * p.ob + d] = (T)(p.gated ? y * (zf * avsi_sigmoid<T>(zf)) : y);
         }
     }
 }

@@ -2,7 +2,8 @@
 arithmetic may add: every function returns (values, bounds), where a bound is the sum of the roundings a float32 evaluation makes on
 its way (U = 2^-24 each), propagated through the recurrences.  Types of 16 bits add their own half step where a value is written.
 
-The constants count operations: a gate (sigmoid, softplus) is at most 8 roundings, a decay exp(delta A) 6 plus what the error of
+The constants count operations: a gate (sigmoid, softplus) is at most 8 roundings (for 16-bit types a sigmoid of x may be |x| of them,
+which stays far inside the half step of what it is rounded to), a decay exp(delta A) 6 plus what the error of
 delta A (8 of delta, 2 of the product, and in a joined chunk the sum over its steps) does to the exponential."""
 import torch
 
