@@ -151,6 +151,7 @@ template <int BITS> __global__ __launch_bounds__(256) void adamw_kernel(Table ta
             topm = avsi_group<64, top_bits>(topm);
             topr = avsi_group<64, top_bits>(topr);
             const float im = block_inv(topm), ir = block_inv(topr);
+            const float least = ir > 0.f ? 0x1p-9f : 0.f;        // (an infinite scale: codes of zero decode to NaN)
             float y[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) y[j] = m[k][j] * im;
@@ -158,7 +159,7 @@ template <int BITS> __global__ __launch_bounds__(256) void adamw_kernel(Table ta
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 y[j] = r[j] * ir;
-                if (r[j] > 0.f && y[j] < 0x1p-9f) y[j] = 0x1p-9f;
+                if (r[j] > 0.f && y[j] < least) y[j] = least;
             }
             store_codes((uint8_t*)t.v + i, n[k], pack4(y));
             if ((threadIdx.x & 63) == 0 && base + k * BLOCK < t.numel) {

@@ -805,7 +805,8 @@ int avsi_selective_scan_step(const avsi_scan_args* args, void* stream);
  *   w -= lr (m / (1 - beta1^step) / (sqrt(v / (1 - beta2^step)) + eps) + weight_decay w); copy = w in its type, if not NULL
  *   bits 32: m, v float.  bits 8: one byte per value, e4m3 codes of m / m_scale and of sqrt(v) / v_scale, where block k of
  *   256 consecutive values of a tensor has the scales m_scale[k] = max|m| / 448, v_scale[k] = max sqrt(v) / 448; a value of
- *   v above zero keeps at least the code of 2^-9.  A block that holds a non-finite moment decodes to NaN.
+ *   v above zero keeps at least the code of 2^-9.  A block of m, or of v, that holds a non-finite value decodes to NaN (that
+ *   moment's: a large finite gradient can make v infinite, (1 - beta2) g^2 > 3.4e38, and leave m finite).
  * `tensors` is a HOST array (read during the call, its pointers are device pointers; numel 0 is skipped, at most
  * 2^36 - 2^12); the tensors must
  * not share memory.  `skip` as for avsi_adam_tf_guarded_f32: with any of its words non-zero nothing is written.
