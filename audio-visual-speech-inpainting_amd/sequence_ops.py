@@ -82,7 +82,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, y=None):
     """(y, mean, rstd): y = (x - mean) * rstd * gamma + beta over the last dimension of x (avsi_layer_norm).
 
     x: any leading shape whose rows lie at one stride (a slice of a wider buffer is fine), unit stride along a row.  gamma, beta:
-    float32 or x's type, either may be None.  y: where to write (x's shape and type; not x itself), allocated if None.  mean, rstd:
+    float32 or x's type, either may be None.  y: where to write (x's shape and type, in memory of its own), allocated if None.  mean, rstd:
     float32, one per row, flat -- what ``layer_norm_bwd`` takes.  A row that holds a NaN or an infinity comes out NaN."""
     M, C, xs = _rows("layer_norm", "x", x)
     _norm_weight("layer_norm", "gamma", gamma, C, x.dtype)
@@ -94,7 +94,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, y=None):
     ys = C
     if y is not None:
         ys = _rows("layer_norm", "y", y, C)[2]
-        if y.shape != x.shape or y.dtype != x.dtype or _overlap(x, y):
+        if y.shape != x.shape or y.dtype != x.dtype or any(t is not None and _overlap(t, y) for t in (x, gamma, beta)):
             _bad("layer_norm: y must have x's shape and type and memory of its own")
     dev = _device("layer_norm", x, gamma, beta, y)
     if y is None:
@@ -110,8 +110,8 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, y=None):
 
 def layer_norm_bwd(dy, x, mean, rstd, gamma=None, want_wgrad=True, dx=None):
     """(dx, dgamma, dbeta) of ``layer_norm`` (avsi_layer_norm_bwd): dy and x of one shape and type, mean and rstd as the forward pass
-    returned them.  dgamma, dbeta: float32 (sums over all rows), None with ``want_wgrad=False``.  dx: where to write, allocated if
-    None."""
+    returned them.  dgamma, dbeta: float32 (sums over all rows), None with ``want_wgrad=False``.  dx: where to write (memory of its own), allocated
+    if None."""
     M, C, xs = _rows("layer_norm_bwd", "x", x)
     dys = _rows("layer_norm_bwd", "dy", dy, C)[2]
     if dy.shape != x.shape or dy.dtype != x.dtype:
@@ -123,7 +123,7 @@ def layer_norm_bwd(dy, x, mean, rstd, gamma=None, want_wgrad=True, dx=None):
     dxs = C
     if dx is not None:
         dxs = _rows("layer_norm_bwd", "dx", dx, C)[2]
-        if dx.shape != x.shape or dx.dtype != x.dtype or _overlap(dx, x) or _overlap(dx, dy):
+        if dx.shape != x.shape or dx.dtype != x.dtype or any(t is not None and _overlap(t, dx) for t in (x, dy, mean, rstd, gamma)):
             _bad("layer_norm_bwd: dx must have x's shape and type and memory of its own")
     dev = _device("layer_norm_bwd", dy, x, mean, rstd, gamma, dx)
     if dx is None:
@@ -242,13 +242,16 @@ def causal_conv_step(x, w, bias=None, silu=True, *, state):
     if D > 1 and x.stride(1) != 1:
         _bad("causal_conv_step: x must have unit stride along its channels")
     _state("causal_conv_step", state, (B, K - 1, D), x.dtype)
-    if _overlap(x, state):
-        _bad("causal_conv_step: x must not be part of the state")
+    lo, size, p = state.data_ptr(), x.element_size(), x.data_ptr()
+    hi = lo + size * B * (K - 1) * D
+    w_at, bias_at = w.data_ptr(), _p(bias)
+    if B and (p < hi and p + size * ((B - 1) * x.stride(0) + D) > lo or w_at < hi and w_at + 4 * D * K > lo
+              or bias_at and bias_at < hi and bias_at + 4 * D > lo):
+        _bad("causal_conv_step: x, w and bias must not be part of the state")
     dev = _device("causal_conv_step", x, w, bias, state)
     y = x.new_empty((B, D))
     if B:
-        _lib.launch_on(dev, "avsi_causal_conv_step", x.data_ptr(), x.stride(0), _CODES[x.dtype], w.data_ptr(), _p(bias), int(silu),
-                       state.data_ptr(), y.data_ptr(), D, B, D, K)
+        _lib.launch_on(dev, "avsi_causal_conv_step", p, x.stride(0), _CODES[x.dtype], w_at, bias_at, int(silu), lo, y.data_ptr(), D, B, D, K)
     return y
 
 
@@ -379,7 +382,8 @@ def selective_scan_bwd(dout, u, dt, A, B, C, D=None, z=None, dt_bias=None, softp
 
 def selective_scan_step(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, *, state):
     """out [batch, channels] of one token per sequence (avsi_selective_scan_step): u, dt, z [batch, channels]; B, C [batch, groups,
-    states] or [batch, states]; ``state`` float32 [batch, channels, states] moves on by one step, in place."""
+    states] or [batch, states]; ``state`` float32 [batch, channels, states] moves on by one step, in place: no other operand may share
+    memory with it."""
     what = "selective_scan_step"
     if u.dim() != 2:
         _bad("%s: u must be [batch, channels]", what)
@@ -388,7 +392,12 @@ def selective_scan_step(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=T
     _state(what, state, (bsz, dim, N), torch.float32)
     lo = state.data_ptr()
     hi = lo + 4 * bsz * dim * N
-    if any(p and lo <= p < hi for p in operands[8:13]):         # (u, dt, z, B, C)
+    (G, _, _, u_at, dt_at, z_at, B_at, C_at, ub, _, tb, _, zb, _, Bb, _, Bg, Cb, _, Cg, A_at, D_at, bias_at) = operands[5:]
+    last, size, vec = bsz - 1, u.element_size(), 4 * dim
+    spans = ((u_at, size * (last * ub + dim)), (dt_at, size * (last * tb + dim)), (z_at, size * (last * zb + dim)),
+             (B_at, size * (last * Bb + (G - 1) * Bg + N)), (C_at, size * (last * Cb + (G - 1) * Cg + N)), (A_at, vec * N), (D_at, vec),
+             (bias_at, vec))
+    if bsz and any(p and p < hi and p + n > lo for p, n in spans):
         _bad("%s: the inputs must not be part of the state", what)
     dev = _device(what, u, dt, A, B, C, D, z, dt_bias, state)
     out = u.new_empty((bsz, dim))
