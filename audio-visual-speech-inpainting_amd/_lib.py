@@ -277,7 +277,9 @@ def lib():
         import torch  # noqa: F401
         handle = ctypes.CDLL(LIB_PATH)
         for name, (restype, argtypes) in PROTOTYPES.items():
-            fn = getattr(handle, name)      # AttributeError if a declared symbol is missing
+            fn = getattr(handle, name, None)
+            if fn is None:                  # (an older build: entry points may be added within an ABI version)
+                raise AvsiError("libavsi_hip.so has no %s, which the host layer expects: rebuild" % name)
             fn.restype = restype
             fn.argtypes = argtypes
         got = handle.avsi_abi_version()
