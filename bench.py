@@ -950,6 +950,55 @@ def self_launch(n):
     return rc if rc >= 0 else 128 - rc
 
 
+def timed_steps(torch, dist, ops, timer, step, steps, warmup, world, shared, device):
+    """(seconds, loss of the last step, fall-backs): `warmup` untimed steps, then exactly `steps` between barriers; the time is the
+    largest over the ranks.
+
+    Ranks that SHARE a GPU (`shared`) can starve each other's cooperative groups into the bounded wait (see the named workloads): then
+    every rank takes the fall-back together and the whole measurement is made again, at most twice.  With a GPU of its own for each
+    rank the first attempt is the only one, and a timeout ends the run."""
+    on = device if world > 1 and dist.get_backend() == "nccl" else "cpu"
+
+    def largest(value, dtype):
+        if world > 1:
+            value = torch.tensor([value], device=on, dtype=dtype)
+            dist.all_reduce(value, op=dist.ReduceOp.MAX)
+            value = value.item()
+        return value
+
+    polls, ops.COOP_POLL_RAISES = ops.COOP_POLL_RAISES, ops.COOP_POLL_RAISES and not shared
+    try:
+        for fallbacks in range(3):
+            for _ in range(warmup):
+                step()
+            timer.reset(steps, warmup)
+            if world > 1:
+                dist.barrier()
+            torch.cuda.synchronize()
+            t0 = time.perf_counter()
+            for _ in range(steps):
+                loss = step()
+            torch.cuda.synchronize()
+            if world > 1:
+                dist.barrier()
+            elapsed = largest(time.perf_counter() - t0, torch.float64)
+            loss = float(loss)
+            try:
+                ops.coop_check(device)
+                late = 0
+            except ops.CoopTimeout:
+                if not shared:
+                    raise
+                late = 1
+            if not (largest(late, torch.int32) if shared else 0):
+                return elapsed, loss, fallbacks
+            if fallbacks < 2:
+                ops.coop_fall_back(device)
+        raise ops.CoopTimeout(ops._COOP_MSG)
+    finally:
+        ops.COOP_POLL_RAISES = polls
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -1055,46 +1104,8 @@ def main():
         _ = model.prediction
         return model.loss_func
 
-    # Ranks that SHARE a GPU can starve each other's cooperative groups into the bounded wait (see the named workloads): then every
-    # rank takes the fall-back together and the whole measurement is made again.  One rank per GPU: the first attempt is the only one.
-    polls, ops.COOP_POLL_RAISES = ops.COOP_POLL_RAISES, ops.COOP_POLL_RAISES and world == 1
-    for attempt in range(3):
-        for _ in range(args.warmup):
-            step()
-        timer.reset(args.steps, args.warmup)
-        if world > 1:
-            dist.barrier()
-        torch.cuda.synchronize()
-        t0 = time.perf_counter()
-        for _ in range(args.steps):
-            loss = step()
-        torch.cuda.synchronize()
-        if world > 1:
-            dist.barrier()
-        elapsed = time.perf_counter() - t0
-        if world > 1:
-            tmax = torch.tensor([elapsed], device=device if dist.get_backend() == "nccl" else "cpu", dtype=torch.float64)
-            dist.all_reduce(tmax, op=dist.ReduceOp.MAX)
-            elapsed = float(tmax.item())
-        loss_val = float(loss)
-        try:
-            ops.coop_check(device)
-            late = 0
-        except ops.CoopTimeout:
-            if world == 1:
-                raise
-            late = 1
-        if world > 1:
-            flag = torch.tensor([late], device=device if dist.get_backend() == "nccl" else "cpu", dtype=torch.int32)
-            dist.all_reduce(flag, op=dist.ReduceOp.MAX)
-            late = int(flag.item())
-        if not late:
-            break
-        if attempt == 2:
-            raise ops.CoopTimeout(ops._COOP_MSG)
-        ops.coop_fall_back(device)
-    ops.COOP_POLL_RAISES = polls
-
+    elapsed, loss_val, fallbacks = timed_steps(torch, dist, ops, timer, step, args.steps, args.warmup, world,
+                                               world > torch.cuda.device_count(), device)
     totals = timer.totals()
     if rank == 0 and train:
         line = {"metric": "training utterances/sec (AV 3xBLSTM-250: front end + forward + BPTT + TF-Adam)",
@@ -1103,7 +1114,7 @@ def main():
                 "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "f32", "data": "synthetic",
                 "config": {"workload": "configs[2]: AV 3xBLSTM-250 training step", "per_gpu_batch": B,
                            "global_batch": B * world, "parallelism": "dp%d" % world},
-                "loss_func": loss_val,
+                "loss_func": loss_val, "coop_fallbacks": fallbacks,
                 "kernel_ms_per_step": {k: v[0] / args.steps for k, v in totals.items()},
                 "calls_ms_last_step": {k: [round(s_.elapsed_time(e_), 2) for s_, e_ in v[-(len(v) // args.steps):]]
                                        for k, v in timer.events.items()}}
@@ -1197,7 +1208,7 @@ def main():
                                    "HIP STFT front end + fp32-MFMA BLSTM forward",
                        "per_gpu_batch": B, "global_batch": B * world, "frames": T_FRAMES, "parallelism": "dp%d" % world},
             "logmel_rms_vs_cpu_oracle": rms,
-            "loss_func": loss_val,
+            "loss_func": loss_val, "coop_fallbacks": fallbacks,
             "roofline": roof,
             "cpu_baseline": cpu,
         }
