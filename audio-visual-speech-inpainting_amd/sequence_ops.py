@@ -174,16 +174,16 @@ def _lengths(what, t, batch):
 def _conv_args(what, x, w, bias, dims):
     if x.dtype not in _CODES or x.dim() != dims:
         _bad("%s: x must be a float32, bfloat16 or float16 tensor of %d dimensions", what, dims)
-    D = x.shape[-1]
-    _fits(what, "sequences", x.shape[0])
-    _fits(what, "channels", D)
-    if dims == 3:
+    B, D = x.shape[0], x.shape[-1]
+    if B > _MOST["sequences"] or D > _MOST["channels"] or dims == 3 and x.shape[1] > _MOST["steps"]:
+        _fits(what, "sequences", B)
+        _fits(what, "channels", D)
         _fits(what, "steps", x.shape[1])
     if w.dim() != 2 or not 2 <= w.shape[1] <= 8 or D < 1:
         _bad("%s: w must be [channels, taps] with 2 to 8 taps", what)
     _vector(what, "w", w, D, w.shape[1])
     _vector(what, "bias", bias, D)
-    return x.shape[0], D, w.shape[1]
+    return B, D, w.shape[1]
 
 
 def causal_conv(x, w, bias=None, silu=True, state=None, lengths=None, want_state=False):
@@ -245,7 +245,7 @@ def causal_conv_step(x, w, bias=None, silu=True, *, state):
     lo, size, p = state.data_ptr(), x.element_size(), x.data_ptr()
     hi = lo + size * B * (K - 1) * D
     w_at, bias_at = w.data_ptr(), _p(bias)
-    if B and (p < hi and p + size * ((B - 1) * x.stride(0) + D) > lo or w_at < hi and w_at + 4 * D * K > lo
+    if lo and B and (p < hi and p + size * ((B - 1) * x.stride(0) + D) > lo or w_at < hi and w_at + 4 * D * K > lo
               or bias_at and bias_at < hi and bias_at + 4 * D > lo):
         _bad("causal_conv_step: x, w and bias must not be part of the state")
     dev = _device("causal_conv_step", x, w, bias, state)
@@ -394,10 +394,12 @@ def selective_scan_step(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=T
     hi = lo + 4 * bsz * dim * N
     (G, _, _, u_at, dt_at, z_at, B_at, C_at, ub, _, tb, _, zb, _, Bb, _, Bg, Cb, _, Cg, A_at, D_at, bias_at) = operands[5:]
     last, size, vec = bsz - 1, u.element_size(), 4 * dim
-    spans = ((u_at, size * (last * ub + dim)), (dt_at, size * (last * tb + dim)), (z_at, size * (last * zb + dim)),
-             (B_at, size * (last * Bb + (G - 1) * Bg + N)), (C_at, size * (last * Cb + (G - 1) * Cg + N)), (A_at, vec * N), (D_at, vec),
-             (bias_at, vec))
-    if bsz and any(p and p < hi and p + n > lo for p, n in spans):
+    if lo and bsz and (u_at < hi and u_at + size * (last * ub + dim) > lo or dt_at < hi and dt_at + size * (last * tb + dim) > lo
+                or z_at and z_at < hi and z_at + size * (last * zb + dim) > lo
+                or B_at < hi and B_at + size * (last * Bb + (G - 1) * Bg + N) > lo
+                or C_at < hi and C_at + size * (last * Cb + (G - 1) * Cg + N) > lo
+                or A_at < hi and A_at + vec * N > lo or D_at and D_at < hi and D_at + vec > lo
+                or bias_at and bias_at < hi and bias_at + vec > lo):
         _bad("%s: the inputs must not be part of the state", what)
     dev = _device(what, u, dt, A, B, C, D, z, dt_bias, state)
     out = u.new_empty((bsz, dim))
