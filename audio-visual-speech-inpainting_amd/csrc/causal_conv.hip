@@ -11,7 +11,7 @@
 // front of them stay in registers, so an input is read once per run and K - 1 inputs again at its start.  In the backward pass the
 // run is followed by K - 1 steps of the next one (dx needs their dpre); the weights' gradients stay in registers over all runs of a
 // thread, are added over a workgroup in LDS and over the workgroups by a second launch, in a fixed order.
-// 8 x 2048 x 2048 bf16, four taps: forward 28 us (4.8 TB/s), backward 48.5 us (4.2 TB/s) and 5 us for the partials; a copy 5.4 TB/s.
+// 8 x 2048 x 2048 bf16, four taps: forward 28 us (4.8 TB/s), backward 49 us (4.1 TB/s) and 5 us for the partials; a copy 5.4 TB/s.
 // Channels in no whole pieces: the last thread takes the last whole piece, which overlaps its neighbour's; both write the same values.
 #include "avsi_common.h"
 #include "avsi_wave.h"

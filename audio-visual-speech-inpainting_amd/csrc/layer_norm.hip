@@ -12,7 +12,7 @@
 // Widths in no whole pieces: the lane that the row's end cuts takes the last whole piece of the row instead, which overlaps its
 // neighbour's; what both hold is counted once and written twice, with the same value.  (A branch around the load would wait for it.)
 //
-// 16384 x 2048 bf16: forward 22.4 us (6.0 TB/s, part of it the Infinity Cache's), backward 38.4 us (5.2 TB/s; a copy of that size 5.4) and
+// 16384 x 2048 bf16: forward 22.7 us (5.9 TB/s, part of it the Infinity Cache's), backward 39 us (5.2 TB/s; a copy of that size 5.4) and
 // 4 us for the partials; 8000 x 512 f32 backward 11.4 + 3.9 us; 32 x 512 f32 2.7 us.
 //
 // Weight gradients: every lane owns the same columns in all its rows, so dgamma and dbeta are sums in its registers; the groups of a

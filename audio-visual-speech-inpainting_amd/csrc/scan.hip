@@ -14,7 +14,7 @@
 // of one channel, N / 4 lanes a channel: four independent chains and one exchange of the sum over the states, in LDS.  Time goes by in
 // tiles of 16 steps, between two kinds of waves (below).  8 sequences of 2048 steps and channels, N = 16, bfloat16: forward 166 us
 // (2.4 TB/s with the states it keeps, the vector unit's counter at 80 %), backward 463 us (81 %); one kind of waves that staged, ran and
-// wrote in turn took 316 and 770 us.
+// wrote in turn took 316 and 770 us.  (float32 operands carry the gates' exponents in two words: 32 x 250 x 512, 23.5 us against 23.0.)
 //
 // Time is cut into chunks only where batch and channels do not fill the chip (chunks_of): then a first launch runs every chunk from a
 // zero state, a second one joins the chunk ends (h_end = exp(A sum delta) h_start + h_local), and the main launch starts from those.
@@ -1014,11 +1014,13 @@ int lanes_of(const avsi_scan_args* a) { return padded(a) / 4; }
 int step_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 int block_channels(int LN) { return LN <= 4 ? 64 : 256 / LN; }
 
-// Chunks of time, of at least 64 steps: as many as give two workgroups to each CU and not one more, so that no CU gets a third; none
-// where batch and channels leave one for three of four CUs -- the launch over the chunks costs three quarters of the main one.  2048 steps, N = 16, a whole forward / backward call in us: 2 sequences of 2048 channels (64 workgroups) 146 / 431
-// uncut, 67 / 158 in 8 chunks (85 / 204 in 6, 79 / 188 in 10); 4 (128) 147 / 439 uncut, 120 / 291 in 4; 6 (192) 152 / 445 uncut,
-// 185 / 514 in 2, 175 / 428 in 4.  Fewer states make smaller workgroups, but no more of them: 8191 steps of 1536 channels with 4 / 8
-// states in 21 chunks 75 / 217 and 94 / 226; in as many as make the waves of 16 states, 85 and 42, 83 / 236 and 98 / 242.
+// Chunks of time, of at least 64 steps: as many as give two workgroups to each CU and not one more; none where batch and channels leave
+// one for three of four CUs -- the launch over the chunks costs three quarters of the main one.  (The forward kernel has room for two
+// workgroups on a CU, so that none gets a third; the backward kernel's LDS, 151552 bytes at 16 states, has room for one, and its two take
+// turns.) 2048 steps, N = 16, a whole forward / backward call in us: 2 sequences of 2048 channels (64 workgroups) 146 / 431 uncut, 67 /
+// 158 in 8 chunks (85 / 204 in 6, 79 / 188 in 10); 4 (128) 147 / 439 uncut, 120 / 291 in 4; 6 (192) 152 / 445 uncut, 185 / 514 in 2, 175 /
+// 428 in 4. Fewer states make smaller workgroups, but no more of them: 8191 steps of 1536 channels with 4 / 8 states in 21 chunks 75 / 217
+// and 94 / 226; in as many as make the waves of 16 states, 85 and 42, 83 / 236 and 98 / 242.
 void chunks_of(const avsi_scan_args* a, int* chunk, int* chunks) {
     const int64_t wgs = (int64_t)a->batch * a->groups * avsi_ceil_div(a->dim / a->groups, block_channels(lanes_of(a)));
     int64_t n = wgs >= 3 * AVSI_NUM_CU / 4 ? 1 : 2 * AVSI_NUM_CU / wgs;

@@ -315,8 +315,9 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, 
     [channels, states], D, dt_bias [channels] float32; D, z, dt_bias may be None.  ``softplus=False`` takes dt + dt_bias as it is.
     state: float32 [batch, channels, states] in front of the first step (None: zeros).  lengths: int32 steps per sequence (clamped to
     0 .. time); behind them out is zero, the state stands still and nothing is read.  new_state (None unless asked for): float32, the
-    state behind each sequence's end.  kept (None unless ``keep``): what ``selective_scan_bwd`` needs, 4 bytes per channel and step
-    at 16 states."""
+    state behind each sequence's end.  kept (None unless ``keep``): what ``selective_scan_bwd`` needs, a quarter of a byte per channel,
+    step and state.  States count as the next power of two from 4 on; with states in no whole quads, or fewer than four channels, as
+    64, here and in the workspace of the backward pass (2 x 4 bytes per state, step and block of 64 channels, of 16 at 64 states)."""
     what = "selective_scan"
     if u.dim() != 3:
         _bad("%s: u must be [batch, time, channels]", what)

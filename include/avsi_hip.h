@@ -773,7 +773,9 @@ int avsi_causal_conv_step(const void* x, int64_t x_stride_b, int dtype, const fl
  *   du, ddt, dz      `dtype` [batch][time][dim] contiguous (dz NULL exactly if z is); dB, dC: `dtype`
  *                    [batch][time][groups][state] contiguous; dA [dim][state], dD [dim], ddt_bias [dim]: float (dD,
  *                    ddt_bias may be NULL)
- * States, sums and statistics are float; every sum has a fixed order.  The step takes one token per sequence (time = 1,
+ * States, sums and statistics are float; every sum has a fixed order.  Memory: states count as the next power of two
+ * from 4 on, as 64 if state is no multiple of 4 or dim < 4.  Gradients that a state enters which is infinite are infinite
+ * or NaN (a product with a zero).  The step takes one token per sequence (time = 1,
  * strides of time unused) and moves the states in `state_out`, which share no memory with the inputs, on in place
  * (state_in, lengths, kept unused).
  * ------------------------------------------------------------------------------------ */
